@@ -35,6 +35,10 @@ COMMON_FLAGS = [
     "-fPIC",
     f"--offload-arch={ARCH}",
     "-munsafe-fp-atomics",
+    # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): the compiler forms it from plain float
+    # code, and some of its forms have given wrong results on gfx950 (the host pass warns that it
+    # does not know the feature: harmless)
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-fvisibility=hidden",
     "-Wno-unused-result",
 ]
@@ -49,7 +53,7 @@ def _newer(target: str, deps: list[str]) -> bool:
 
 def _tag(extra: list[str]) -> str:
     import hashlib
-    return hashlib.sha1(" ".join(extra).encode()).hexdigest()[:8]
+    return hashlib.sha1(" ".join(COMMON_FLAGS + extra).encode()).hexdigest()[:8]
 
 
 # per-unit flags (measured choices, see the unit's header comment)
