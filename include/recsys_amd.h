@@ -845,6 +845,72 @@ int rs_ctr_metrics_accumulate(void* stream, const float* p, int64_t p_ld, const 
                               double* state);
 int rs_ctr_metrics_result(void* stream, const double* state, int nthr, float* out);
 
+/* ---------------------------------------------------------------------------------------
+ * Sequence operators: layer normalisation, the gated linear recurrence and 8-bit activation
+ * checkpoints (recommendsystem_amd/sequence.py).  The reference reads behaviour sequences by
+ * pooling only (din.py:18-47, staytime/layer.py:16-41) and takes its LayerNormalization from a
+ * module it does not hold (InteractingLayer.py:5); these read a history in order.
+ *
+ * dtype: element type of the rows: 0 fp32, 1 bf16, 2 fp16.  Everything else named float (gamma,
+ * beta, statistics, states, parameter gradients) is fp32; all sums and states are held in fp32
+ * and rounded once, on the store.  Rows have unit stride along D; ld_* / *_sb / *_st count
+ * elements, rows may start at any element and input strides may be 0.
+ * ------------------------------------------------------------------------------------- */
+#define RS_DTYPE_F32 0
+#define RS_DTYPE_BF16 1
+#define RS_DTYPE_F16 2
+
+/* 8-bit form of x [rows, D] (contiguous codes [rows, D], scales [rows, ceil(D / 128)]): in each
+ * block of 128 columns scale = max|x| / 127 in fp32 and code = x / scale to the nearest whole
+ * number, ties to even.  A block with max|x| < 2^-100 reads back as zeros, one that holds an
+ * infinity or NaN as NaN.  rs_unpack8: y = code * scale. */
+int rs_pack8(void* stream, int dtype, const void* x, int64_t ld_x, int64_t rows, int D,
+             int8_t* codes, float* scales);
+int rs_unpack8(void* stream, int dtype, const int8_t* codes, const float* scales, int64_t rows,
+               int D, void* y, int64_t ld_y);
+
+/* y = (x - mean) rstd gamma + beta, rstd = 1 / sqrt(var + eps), over the last axis, D <= 32768
+ * (larger: -2), eps > 0.  mean / rstd [rows] for the backward (both or neither); codes / scales
+ * (both or neither): the 8-bit form of x, written in the same pass. */
+int rs_layernorm_fwd(void* stream, int dtype, const void* x, int64_t ld_x, int64_t rows, int D,
+                     const float* gamma, const float* beta, float eps, void* y, int64_t ld_y,
+                     float* mean, float* rstd, int8_t* codes, float* scales);
+/* dx [rows, D], dgamma [D], dbeta [D] (accumulate: added onto).  The input is x or its 8-bit form
+ * (codes and scales; x NULL then); mean / rstd are the forward's.  rows = 0 leaves zero parameter
+ * gradients.  The sums over rows run in an order fixed by the shape. */
+int64_t rs_layernorm_bwd_workspace_floats(int64_t rows, int D);
+int rs_layernorm_bwd(void* stream, int dtype, const void* dy, int64_t ld_dy, const void* x,
+                     int64_t ld_x, const int8_t* codes, const float* scales, int64_t rows, int D,
+                     const float* gamma, const float* mean, const float* rstd, void* dx,
+                     int64_t ld_dx, float* dgamma, float* dbeta, int accumulate, float* workspace,
+                     int64_t workspace_floats);
+
+/* h_t = f_t h_{t-1} + (1 - f_t) v_t, f_t = sigmoid(g_t), for v, g [B, T, D] (batch stride *_sb,
+ * step stride *_st).  h0 [B, D] (NULL: zeros).  lengths int32 [B] (NULL: T everywhere; values are
+ * taken into 0..T): steps behind them are not read, h is zero there and the state stands still.
+ * h [B, T, D] contiguous; last [B, D]: the state after lengths[b] steps.  states
+ * (rs_gated_rec_states_floats; NULL without a backward): fp32 states at fixed steps, for
+ * rs_gated_rec_bwd with the same shape.  workspace: rs_gated_rec_workspace_floats floats. */
+int64_t rs_gated_rec_states_floats(int dtype, int64_t B, int64_t T, int D);
+int64_t rs_gated_rec_workspace_floats(int dtype, int64_t B, int64_t T, int D);
+int rs_gated_rec_fwd(void* stream, int dtype, const void* v, int64_t v_sb, int64_t v_st,
+                     const void* g, int64_t g_sb, int64_t g_st, int64_t B, int64_t T, int D,
+                     const int32_t* lengths, const float* h0, void* h, float* last, float* states,
+                     float* workspace, int64_t workspace_floats);
+/* dv, dg [B, T, D] (strided, zero behind lengths; the halves of one [B, T, 2 D] buffer, say), dh0
+ * [B, D] (nullable) from dh [B, T, D] (NULL: zeros) and dlast [B, D] (NULL: zeros). */
+int rs_gated_rec_bwd(void* stream, int dtype, const void* v, int64_t v_sb, int64_t v_st,
+                     const void* g, int64_t g_sb, int64_t g_st, int64_t B, int64_t T, int D,
+                     const int32_t* lengths, const float* states, const void* dh, int64_t dh_sb,
+                     int64_t dh_st, const float* dlast, void* dv, int64_t dv_sb, int64_t dv_st,
+                     void* dg, int64_t dg_sb, int64_t dg_st, float* dh0, float* workspace,
+                     int64_t workspace_floats);
+/* One step for B tokens: v, g [B, D] (row strides ld_*), state [B, D] fp32 (NULL: zeros) ->
+ * h [B, D] in the rows' type and new_state [B, D] fp32 (may be state itself). */
+int rs_gated_rec_step(void* stream, int dtype, const void* v, int64_t ld_v, const void* g,
+                      int64_t ld_g, int64_t B, int D, const float* state, void* h,
+                      float* new_state);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,8 @@ from .embedding import (EmbeddingFeatures, SequenceEmbedding, SparseAdaGrad, Spa
                         SparseTable)
 from .din import DIN, StaytimeDIN  # noqa: F401
 from .layers import Dense, InteractingLayer, MultiLayerDense  # noqa: F401
+from .sequence import (GatedRecurrence, LayerNormalization, SequenceEncoder,  # noqa: F401
+                       gated_recurrence, gated_recurrence_step, layer_norm, pack8, unpack8)
 from .autoint import AutoInt, AutoIntConfig, AutoIntTrainer, cross_entropy  # noqa: F401
 
 __version__ = "0.1.0"

@@ -102,6 +102,21 @@ SIGNATURES: dict[str, tuple] = {
                              _i32]),
     "rs_dense_adam_done": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _f32, _f32, _f32, _f32, _f32,
                              _i32, _vp]),
+    "rs_pack8": (_i32, [_vp, _i32, _vp, _i64, _i64, _i32, _vp, _vp]),
+    "rs_unpack8": (_i32, [_vp, _i32, _vp, _vp, _i64, _i32, _vp, _i64]),
+    "rs_layernorm_fwd": (_i32, [_vp, _i32, _vp, _i64, _i64, _i32, _vp, _vp, _f32, _vp, _i64, _vp,
+                                _vp, _vp, _vp]),
+    "rs_layernorm_bwd_workspace_floats": (_i64, [_i64, _i32]),
+    "rs_layernorm_bwd": (_i32, [_vp, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _vp,
+                                _vp, _vp, _i64, _vp, _vp, _i32, _vp, _i64]),
+    "rs_gated_rec_states_floats": (_i64, [_i32, _i64, _i64, _i32]),
+    "rs_gated_rec_workspace_floats": (_i64, [_i32, _i64, _i64, _i32]),
+    "rs_gated_rec_fwd": (_i32, [_vp, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp,
+                                _vp, _vp, _vp, _vp, _vp, _i64]),
+    "rs_gated_rec_bwd": (_i32, [_vp, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp,
+                                _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                                _i64]),
+    "rs_gated_rec_step": (_i32, [_vp, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
     "rs_din_param_count": (_i32, [_i32, _i32]),
     "rs_din_bwd_workspace_floats": (_i64, [_i32, _i64, _i32, _i32]),
     "rs_din_fwd": (_i32, [_vp, _i32, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _i32,

@@ -19,6 +19,7 @@ from torch import nn
 
 from . import _lib
 from ._lib import call, ptr, stream_handle
+from .packing import pack8, unpack8
 from .params import FlatBlock, glorot_uniform_, grads_contiguous
 
 ACTIVATIONS = {None: 0, "linear": 0, "relu": 1, "sigmoid": 2}
@@ -268,8 +269,10 @@ def gather_multi(src, plans):
 
 
 class _DenseFn(torch.autograd.Function):
+    """save_8bit: x is kept for the backward as pack8's codes and scales."""
+
     @staticmethod
-    def forward(ctx, x, W, b, act, sink=None):
+    def forward(ctx, x, W, b, act, sink=None, save_8bit=False):
         _lib.require_device(x, W)
         x = _row_major(x)
         M, K = x.shape
@@ -277,14 +280,16 @@ class _DenseFn(torch.autograd.Function):
         y = torch.empty(M, N, device=x.device, dtype=torch.float32)
         call("rs_dense_fwd", stream_handle(), ptr(x), M, K, x.stride(0), ptr(W), ptr(b), N, act,
              ptr(y), N)
-        ctx.save_for_backward(x, y, W, b)
+        ctx.save_for_backward(*(pack8(x) if save_8bit else (x, None)), y, W, b)
         ctx.act = act
         ctx.sink = sink
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, y, W, b = ctx.saved_tensors
+        x, scales, y, W, b = ctx.saved_tensors
+        if scales is not None:
+            x = unpack8(x, scales)
         dy = _row_major(dy)
         M, K = x.shape
         N = W.shape[1]
@@ -311,19 +316,22 @@ class _DenseFn(torch.autograd.Function):
             call("rs_dense_bwd_weight", s, ptr(x), x.stride(0), ptr(dy), dy.stride(0), ptr(y), N,
                  ctx.act, M, K, N, ptr(dW), ptr(db), 1 if in_place else 0, ptr(ws), ws_n)
         if in_place:
-            return dx, None, None, None, None
-        return dx, dW, db, None, None
+            return dx, None, None, None, None, None
+        return dx, dW, db, None, None, None
 
 
 class Dense(nn.Module):
-    """tf.keras.layers.Dense(units, activation): glorot_uniform kernel [in, units], zero bias."""
+    """tf.keras.layers.Dense(units, activation): glorot_uniform kernel [in, units], zero bias.
+    save_8bit: keep the input for the backward in 8 bits (packing.py); the outputs and the input's
+    gradient do not change, the kernel's gradient is that of the kept values."""
 
-    def __init__(self, units, activation=None, seed=0, device=None, name=None):
+    def __init__(self, units, activation=None, seed=0, device=None, name=None, save_8bit=False):
         super().__init__()
         self.units = int(units)
         self.activation = activation
         self.act = _act_code(activation)
         self.seed = int(seed)
+        self.save_8bit = bool(save_8bit)
         self._device = device
         self.built = False
         self.name = name
@@ -344,11 +352,11 @@ class Dense(nn.Module):
             self.build(tuple(x.shape), device=x.device)
         lead = x.shape[:-1]  # Keras Dense = tensordot over the last axis
         from . import ops
-        if ops.custom_ops_enabled():
+        if ops.custom_ops_enabled() and not self.save_8bit:
             y = torch.ops.ctr.dense(x.reshape(-1, x.shape[-1]).float(), self.kernel, self.bias, self.act)
             return y.reshape(*lead, self.units)
         y = _DenseFn.apply(x.reshape(-1, x.shape[-1]).float(), self.kernel, self.bias, self.act,
-                           grad_sink)
+                           grad_sink, self.save_8bit and torch.is_grad_enabled())
         return y.reshape(*lead, self.units)
 
 
@@ -426,9 +434,9 @@ class _GroupedDenseFn(torch.autograd.Function):
 def grouped_dense(layers, xs):
     """[layer_i(x_i)] for built Dense layers of one input rank, as ONE grouped launch per pass
     (same math as calling each layer; the per-expert / per-task loops of staytime/VideoDnn.py and
-    rough_rank/layer.py).  Up to 8 layers per group."""
+    rough_rank/layer.py).  Up to 8 layers per group; layers with save_8bit run one by one."""
     layers, xs = list(layers), list(xs)
-    if len(layers) == 1 or len(layers) > 8:
+    if len(layers) == 1 or len(layers) > 8 or any(l.save_8bit for l in layers):
         return [l(x) for l, x in zip(layers, xs)]
     for l, x in zip(layers, xs):
         if not l.built:

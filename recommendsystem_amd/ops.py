@@ -13,6 +13,9 @@ kernels:
     ctr::embedding_lookup                         EmbeddingFeatures forward (rank/ctr/base_model.py:
                                                   203-217); its sparse push is the table's
                                                   (embedding.SparseTable), not an autograd output
+    ctr::layer_norm / ctr::layer_norm_bwd         sequence.layer_norm
+    ctr::gated_recurrence / _bwd                  sequence.gated_recurrence
+    ctr::pack8 / ctr::unpack8                     packing.pack8 / unpack8 (no autograd formula)
 
 The layer classes (layers.InteractingLayer, din.DIN, layers.Dense) keep their in-place gradient
 fast path (autograd.Function writing into the flat parameter block); ``use_custom_ops(True)``
@@ -26,7 +29,7 @@ import torch
 from torch import Tensor
 from torch.library import custom_op
 
-from . import _lib
+from . import _lib, packing, sequence
 from ._lib import call, ptr, stream_handle
 
 _U64 = 0xFFFFFFFFFFFFFFFF
@@ -309,3 +312,128 @@ def _(ids, offsets, row_base, bucket, hash_mode, combiner, table):
     else:
         B = (offsets.shape[0] - 1) // F
     return table.new_empty(B, F, table.shape[1]), ids.new_empty(ids.numel(), dtype=torch.int32)
+
+
+# ============================================================================================
+# sequence operators (sequence.py)
+# ============================================================================================
+@custom_op("ctr::layer_norm", mutates_args=())
+def layer_norm(x: Tensor, gamma: Tensor, beta: Tensor, epsilon: float) -> tuple[Tensor, Tensor, Tensor]:
+    """(y, mean, rstd) of sequence.layer_norm."""
+    code = sequence._check_norm(x, gamma, beta, epsilon)
+    with packing.on_device(x, gamma, beta):
+        return sequence._norm_forward(x, gamma, beta, epsilon, code, True, False)[:3]
+
+
+@layer_norm.register_fake
+def _(x, gamma, beta, epsilon):
+    rows = x.numel() // x.shape[-1]
+    return (x.new_empty(x.shape), x.new_empty(rows, dtype=torch.float32),
+            x.new_empty(rows, dtype=torch.float32))
+
+
+@custom_op("ctr::layer_norm_bwd", mutates_args=())
+def layer_norm_bwd(dy: Tensor, x: Tensor, gamma: Tensor, mean: Tensor,
+                   rstd: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+    with packing.on_device(dy, x, gamma, mean, rstd):
+        dx = sequence._norm_backward(dy, x, None, None, gamma, mean, rstd,
+                                     packing.element_code(x, "layer_norm's input"), dgamma, dbeta, False)
+    return dx, dgamma, dbeta
+
+
+@layer_norm_bwd.register_fake
+def _(dy, x, gamma, mean, rstd):
+    return dy.new_empty(dy.shape), torch.empty_like(gamma), torch.empty_like(gamma)
+
+
+def _ln_setup(ctx, inputs, output):
+    x, gamma, _, _ = inputs
+    ctx.save_for_backward(x, gamma, output[1], output[2])
+
+
+def _ln_backward(ctx, dy, _dmean, _drstd):
+    return (*torch.ops.ctr.layer_norm_bwd(dy, *ctx.saved_tensors), None)
+
+
+layer_norm.register_autograd(_ln_backward, setup_context=_ln_setup)
+
+
+def _rec_sizes(v, g):
+    return v.shape[0], v.shape[1], v.shape[2] if g is not None else v.shape[2] // 2
+
+
+@custom_op("ctr::gated_recurrence", mutates_args=())
+def gated_recurrence(v: Tensor, g: Optional[Tensor], h0: Optional[Tensor],
+                     lengths: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
+    """(h, last, states) of sequence.gated_recurrence; states are the backward's."""
+    code = sequence._check_rec(v, g, 3, "gated_recurrence")
+    B, T, D = _rec_sizes(v, g)
+    sequence._check_state(h0, (B, D), "gated_recurrence: h0")
+    with packing.on_device(v, g, h0, lengths):
+        return sequence._rec_forward(v, g, h0.contiguous() if h0 is not None else None,
+                                     sequence._check_lengths(lengths, B, T), code, True)
+
+
+@gated_recurrence.register_fake
+def _(v, g, h0, lengths):
+    B, T, D = _rec_sizes(v, g)
+    code = packing.element_code(v, "gated_recurrence's values")
+    n = int(_lib.load().rs_gated_rec_states_floats(code, B, T, D))
+    return (v.new_empty(B, T, D), v.new_empty(B, D, dtype=torch.float32),
+            v.new_empty(n, dtype=torch.float32))
+
+
+@custom_op("ctr::gated_recurrence_bwd", mutates_args=())
+def gated_recurrence_bwd(dh: Tensor, dlast: Tensor, v: Tensor, g: Optional[Tensor],
+                         lengths: Optional[Tensor], states: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    """(dv, dg, dh0); with g None dv is the joint rows' gradient and dg is empty."""
+    B, T, D = _rec_sizes(v, g)
+    with packing.on_device(v, g, dh, dlast, lengths, states):
+        dv, dg, dh0 = sequence._rec_backward(v, g, sequence._check_lengths(lengths, B, T), states, dh,
+                                             dlast, packing.element_code(v, "gated_recurrence's values"),
+                                             True)
+    return dv, v.new_empty(0) if dg is None else dg, dh0
+
+
+@gated_recurrence_bwd.register_fake
+def _(dh, dlast, v, g, lengths, states):
+    return (v.new_empty(v.shape), v.new_empty(0) if g is None else v.new_empty(v.shape),
+            torch.empty_like(dlast))
+
+
+def _rec_setup(ctx, inputs, output):
+    v, g, h0, lengths = inputs
+    ctx.save_for_backward(v, g, lengths, output[2])
+    ctx.has_g, ctx.has_h0 = g is not None, h0 is not None
+
+
+def _rec_op_backward(ctx, dh, dlast, _dstates):
+    v, g, lengths, states = ctx.saved_tensors
+    dv, dg, dh0 = torch.ops.ctr.gated_recurrence_bwd(dh, dlast, v, g, lengths, states)
+    return dv, dg if ctx.has_g else None, dh0 if ctx.has_h0 else None, None
+
+
+gated_recurrence.register_autograd(_rec_op_backward, setup_context=_rec_setup)
+
+
+@custom_op("ctr::pack8", mutates_args=())
+def pack8(x: Tensor) -> tuple[Tensor, Tensor]:
+    """(codes, scales) of packing.pack8."""
+    return packing.pack8(x)
+
+
+@pack8.register_fake
+def _(x):
+    return (x.new_empty(x.shape, dtype=torch.int8),
+            x.new_empty(packing.scale_shape(x.shape), dtype=torch.float32))
+
+
+@custom_op("ctr::unpack8", mutates_args=())
+def unpack8(codes: Tensor, scales: Tensor, dtype: torch.dtype) -> Tensor:
+    return packing.unpack8(codes, scales, dtype)
+
+
+@unpack8.register_fake
+def _(codes, scales, dtype):
+    return codes.new_empty(codes.shape, dtype=dtype)

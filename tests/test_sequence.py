@@ -1,0 +1,133 @@
+"""CPU: the sequence operators' refusals (all of them raise before anything is launched), size
+queries and meta shapes."""
+import pytest
+import torch
+
+from recommendsystem_amd import _lib, packing, sequence
+from recommendsystem_amd import ops  # noqa: F401
+from recommendsystem_amd.layers import Dense
+
+F32, BF16, F16, F64 = torch.float32, torch.bfloat16, torch.float16, torch.float64
+E = torch.empty
+
+
+@pytest.mark.parametrize("call, error, text", [
+    (lambda: sequence.layer_norm(E(3, 4, dtype=F64), E(4), E(4)), TypeError, "float32, bfloat16"),
+    (lambda: sequence.layer_norm(E(()), E(4), E(4)), ValueError, "last dimension"),
+    (lambda: sequence.layer_norm(E(3, 0), E(0), E(0)), ValueError, "last dimension"),
+    (lambda: sequence.layer_norm(E(1, 32769), E(32769), E(32769)), ValueError, "1 to 32768"),
+    (lambda: sequence.layer_norm(E(3, 4), E(5), E(4)), ValueError, "gamma"),
+    (lambda: sequence.layer_norm(E(3, 4), E(4), E(1, 4)), ValueError, "beta"),
+    (lambda: sequence.layer_norm(E(3, 4, dtype=BF16), E(4, dtype=BF16), E(4)), TypeError, "gamma"),
+    (lambda: sequence.layer_norm(E(3, 4), E(4), E(4), 0.0), ValueError, "epsilon"),
+    (lambda: sequence.layer_norm(E(3, 4), E(4), E(4), float("nan")), ValueError, "epsilon"),
+    (lambda: sequence.gated_recurrence(E(2, 3), E(2, 3)), ValueError, "rank-3"),
+    (lambda: sequence.gated_recurrence(E(2, 3, 4), E(2, 3, 5)), ValueError, "differ in shape"),
+    (lambda: sequence.gated_recurrence(E(2, 3, 4), E(2, 3, 4, dtype=F16)), TypeError, "differ in type"),
+    (lambda: sequence.gated_recurrence(E(2, 3, 4, dtype=torch.int32), E(2, 3, 4)), TypeError, "values"),
+    (lambda: sequence.gated_recurrence(E(2, 3, 0), E(2, 3, 0)), ValueError, "last dimension"),
+    (lambda: sequence.gated_recurrence(E(2, 3, 5)), ValueError, "even"),
+    (lambda: sequence.gated_recurrence(E(2, 3, 0)), ValueError, "even"),
+    (lambda: sequence.gated_recurrence(E(2, 3, 4), E(2, 3, 4), E(2, 5)), ValueError, "h0"),
+    (lambda: sequence.gated_recurrence(E(2, 3, 4), E(2, 3, 4), E(2, 4, dtype=BF16)), TypeError, "h0"),
+    (lambda: sequence.gated_recurrence_step(E(2, 3, 4), E(2, 3, 4)), ValueError, "rank-2"),
+    (lambda: sequence.gated_recurrence_step(E(2, 4), E(2, 4), E(3, 4)), ValueError, "state"),
+    (lambda: sequence.gated_recurrence_step(E(2, 4), E(2, 4), None, E(4, 2).t()), ValueError, "contiguous"),
+    (lambda: sequence.gated_recurrence_step(E(2, 4, requires_grad=True), E(2, 4)), RuntimeError, "no backward"),
+    (lambda: sequence.pack8(E(3, 4, dtype=torch.int32)), TypeError, "float32"),
+    (lambda: sequence.pack8(E(3, 0)), ValueError, "last dimension"),
+    (lambda: sequence.unpack8(E(3, 4), E(3, 1)), TypeError, "int8"),
+    (lambda: sequence.unpack8(E(3, 4, dtype=torch.int8), E(3, 2)), ValueError, "do not fit"),
+    (lambda: sequence.unpack8(E(3, 4, dtype=torch.int8), E(3, 1), F64), TypeError, "dtype"),
+    (lambda: sequence.GatedRecurrence(0), ValueError, "unit"),
+    (lambda: sequence.GatedRecurrence(4)(E(2, 3)), ValueError, "rank of input"),
+    (lambda: sequence.SequenceEncoder(4, depth=0), ValueError, "depth"),
+    (lambda: sequence.SequenceEncoder(4)(E(2, 3)), ValueError, "rank of input"),
+    (lambda: sequence.SequenceEncoder(4)(E(2, 3, 5), None, E(1, 2, 5)), ValueError, "states"),
+])
+def test_refusals(call, error, text):
+    with pytest.raises(error, match=text):
+        call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: sequence.layer_norm(E(3, 4), E(4), E(4)),
+    lambda: sequence.gated_recurrence(E(2, 3, 4), E(2, 3, 4)),
+    lambda: sequence.gated_recurrence_step(E(2, 4), E(2, 4)),
+    lambda: sequence.pack8(E(3, 4)),
+    lambda: sequence.unpack8(E(3, 4, dtype=torch.int8), E(3, 1)),
+])
+def test_no_cpu_fallback(call):
+    with pytest.raises(_lib.RecsysKernelError, match="ROCm device"):
+        call()
+
+
+def test_lengths_checks():
+    for bad, err in ((E(3), TypeError), (E(4, dtype=torch.int32), ValueError),
+                     (E(3, 1, dtype=torch.int32), ValueError)):
+        with pytest.raises(err, match="lengths"):
+            sequence._check_lengths(bad, 3, 5)
+    got = sequence._check_lengths(torch.tensor([2 ** 32 + 1, -7, 3]), 3, 5)
+    assert got.dtype == torch.int32 and got.tolist() == [5, 0, 3]
+
+
+def test_entry_points_reject():
+    """The C entry points refuse what they cannot run before they launch (null or short buffers)."""
+    lib = _lib.load()
+    some = torch.zeros(64)
+    p = some.data_ptr()
+    ARG, UNS = _lib.RS_ERR_ARG, _lib.RS_ERR_UNSUPPORTED
+    assert lib.rs_pack8(None, 3, p, 4, 1, 4, p, p) == ARG           # type
+    assert lib.rs_pack8(None, 0, None, 4, 1, 4, p, p) == ARG
+    assert lib.rs_pack8(None, 0, p, 4, 1, 0, p, p) == ARG
+    assert lib.rs_pack8(None, 0, None, 4, 0, 4, None, None) == 0    # no rows
+    assert lib.rs_unpack8(None, 0, p, p, 1, 4, p, 3) == ARG         # ld_y < D
+    assert lib.rs_layernorm_fwd(None, 0, p, 4, 1, 32769, p, p, 1e-5, p, 32769, None, None, None, None) == UNS
+    assert lib.rs_layernorm_fwd(None, 0, p, 4, 1, 4, p, p, 0.0, p, 4, None, None, None, None) == ARG
+    assert lib.rs_layernorm_fwd(None, 0, p, 4, 1, 4, p, p, 1e-5, p, 4, p, None, None, None) == ARG
+    assert lib.rs_layernorm_fwd(None, 0, p, 4, 1, 4, p, p, 1e-5, p, 4, None, None, p, None) == ARG
+    need = lib.rs_layernorm_bwd_workspace_floats(1000, 4)
+    assert lib.rs_layernorm_bwd(None, 0, p, 4, p, 4, None, None, 1000, 4, p, p, p, p, 4, p, p, 0, p, need - 1) == ARG
+    assert lib.rs_layernorm_bwd(None, 0, p, 4, p, 4, p, p, 1, 4, p, p, p, p, 4, p, p, 0, p, 64) == ARG  # both
+    assert lib.rs_gated_rec_fwd(None, 0, p, 4, 4, p, 4, 4, 1, -1, 4, None, None, p, p, None, None, 0) == ARG
+    assert lib.rs_gated_rec_fwd(None, 0, p, 4, 4, p, 4, 4, 1, 1, 4, None, None, p, None, None, None, 0) == ARG
+    assert lib.rs_gated_rec_fwd(None, 0, p, 4, 4, p, 4, 4, 0, 9, 4, None, None, None, None, None, None, 0) == 0
+    assert lib.rs_gated_rec_bwd(None, 0, p, 4, 4, p, 4, 4, 1, 1, 4, None, None, p, 4, 4, p, p, 4, 4, p, 4, 4,
+                                p, None, 0) == ARG                   # no states
+    assert lib.rs_gated_rec_step(None, 0, p, 4, p, 4, 1, 4, p, p, None) == ARG
+    # a workspace that the shape needs and that is missing
+    B, T, D = 1, 1 << 20, 8
+    if lib.rs_gated_rec_workspace_floats(0, B, T, D):
+        assert lib.rs_gated_rec_fwd(None, 0, p, 8, 8, p, 8, 8, B, T, D, None, None, p, p, None, None, 0) == ARG
+
+
+def test_size_queries():
+    lib = _lib.load()
+    for B, T, D in ((1, 1, 1), (3, 50, 32), (1, 1 << 20, 1000), (70000, 3, 5), (8, 4096, 2048)):
+        for code in (0, 1, 2):
+            assert 0 <= lib.rs_gated_rec_states_floats(code, B, T, D) <= B * T * D
+            assert lib.rs_gated_rec_workspace_floats(code, B, T, D) >= 0
+    assert lib.rs_gated_rec_states_floats(0, -1, 5, 5) == 0
+    assert lib.rs_gated_rec_states_floats(7, 1, 5, 5) == 0
+    assert lib.rs_layernorm_bwd_workspace_floats(-1, 5) == 0
+
+
+def test_meta_shapes():
+    m = dict(device="meta")
+    x, p = E(4, 5, 300, dtype=BF16, **m), E(300, **m)
+    y, mean, rstd = torch.ops.ctr.layer_norm(x, p, p, 1e-5)
+    assert y.shape == x.shape and y.dtype == BF16 and mean.shape == rstd.shape == (20,)
+    dx, dg, db = torch.ops.ctr.layer_norm_bwd(y, x, p, mean, rstd)
+    assert dx.shape == x.shape and dg.shape == db.shape == (300,) and dg.dtype == F32
+    h, last, states = torch.ops.ctr.gated_recurrence(x, None, None, None)
+    assert h.shape == (4, 5, 150) and last.shape == (4, 150) and last.dtype == F32
+    dv, dgt, dh0 = torch.ops.ctr.gated_recurrence_bwd(h, last, x, None, None, states)
+    assert dv.shape == x.shape and dgt.numel() == 0 and dh0.shape == (4, 150)
+    codes, scales = torch.ops.ctr.pack8(x)
+    assert codes.shape == x.shape and codes.dtype == torch.int8 and scales.shape == (4, 5, 3)
+    assert torch.ops.ctr.unpack8(codes, scales, F16).dtype == F16
+
+
+def test_dense_flag_defaults_off():
+    assert not Dense(3).save_8bit and Dense(3, save_8bit=True).save_8bit
+    assert packing.scale_shape((2, 129)) == (2, 2)
