@@ -11,7 +11,8 @@ rounded once: half(t) |value|.  Below fp16's normal range (2^-14) the step is fi
   * recurrence: the error of a state obeys the recurrence itself, e_t = f_t e_{t-1} + what step t
     adds: 2 u for each of its roundings and 4 u of its input for the gate (exp and reciprocal),
     taken as 16 u of the magnitudes, which also covers joining partial results in another order
-    (each join rounds values of the same magnitude, and a step lies under at most 16 joins).
+    (each join rounds values no larger than the sum of the magnitudes of the state's terms, and a
+    step lies under at most 16 joins).
 """
 from __future__ import annotations
 
@@ -258,11 +259,13 @@ def ref_rec(v, g, h0, lengths, dh=None, dlast=None):
     i = torch.where(live, torch.sigmoid(-g), torch.zeros(()).double())
     f = torch.where(live, torch.sigmoid(g), torch.ones(()).double())
     s = h0.double().cpu() if h0 is not None else torch.zeros(B, D).double()
-    e = torch.zeros(B, D).double()
+    e, top = torch.zeros(B, D).double(), s.abs()
     hs, es = [s], [e]
     for t in range(T):
         new = s + i[:, t] * (v[:, t] - s)
-        add = 16 * U * (new.abs() + s.abs() + i[:, t] * (v[:, t].abs() + s.abs()))
+        # (top: the sum of the magnitudes of h's terms, which partial results are as large as)
+        top = torch.where(live[:, t], f[:, t] * top + i[:, t] * v[:, t].abs(), top)
+        add = 16 * U * (new.abs() + top + i[:, t] * (v[:, t].abs() + s.abs()))
         e = torch.where(live[:, t], f[:, t] * e + add, e)
         s = torch.where(live[:, t], new, s)
         hs.append(s)
@@ -274,7 +277,7 @@ def ref_rec(v, g, h0, lengths, dh=None, dlast=None):
         return out
     r = dlast.double().cpu() if dlast is not None else torch.zeros(B, D).double()
     dh = dh.double().cpu() if dh is not None else torch.zeros(B, T, D).double()
-    er = torch.zeros(B, D).double()
+    er, big = torch.zeros(B, D).double(), r.abs()
     dv, dg, bv, bg = (torch.zeros(B, T, D).double() for _ in range(4))
     for t in range(T - 1, -1, -1):
         on = live[:, t]
@@ -287,7 +290,10 @@ def ref_rec(v, g, h0, lengths, dh=None, dlast=None):
         # the factor 1 - i is off by an absolute u beside its own rounding
         bg[:, t] = torch.where(on, i[:, t] * (f[:, t] * (ea * d.abs() + a.abs() * EH[:, t] + 16 * U * (a * d).abs())
                                               + 4 * U * (a * d).abs()), zero)
-        er = torch.where(on, f[:, t] * ea + 8 * U * a.abs(), er)
+        # r is joined from partial results that are as large as the sum of its terms' magnitudes,
+        # whatever r itself cancels to: er obeys the recurrence with |dh| + the magnitude so far
+        big = torch.where(on, f[:, t] * (big + dh[:, t].abs()), big)
+        er = torch.where(on, f[:, t] * ea + 8 * U * (a.abs() + big), er)
         r = torch.where(on, f[:, t] * a, r)
     return out + [(dv, bv), (dg, bg), (r, er)]
 
@@ -378,6 +384,19 @@ def test_recurrence_extreme_gates(dtype):
         got = (h, last, *torch.autograd.grad(h, (vr, g), dh))
         for a, (w, b), what in zip(got, ref_rec(v, g.detach(), h0, None, dh), ("h", "last", "dv", "dg")):
             near(a, w, b + 1e-38, f"{what} at gate {gate}")
+
+
+def test_recurrence_large_state_is_forgotten():
+    """A state of 10^6 in front of values around 1, half of it forgotten a step: its rounding is
+    forgotten with it, in the states and (from the other end) in the gradients."""
+    B, T, D = 1, 700, 16
+    v, g, dh = rnd(B, T, D), rnd(B, T, D, std=0.1).requires_grad_(), rnd(B, T, D)
+    h0, dlast = 1e6 * rnd(B, D), 1e6 * rnd(B, D)
+    vr = v.clone().requires_grad_()
+    h, last = gated_recurrence(vr, g, h0)
+    got = (h, last, *torch.autograd.grad((h, last), (vr, g), (dh, dlast)))
+    for a, (w, b) in zip(got, ref_rec(v, g.detach(), h0, None, dh, dlast)):
+        near(a, w, b, "large state")
 
 
 def test_recurrence_nan_stays_in_its_channel():
