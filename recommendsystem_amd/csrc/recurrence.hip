@@ -55,83 +55,6 @@ template <> struct ShutGate<ElemF32> { static constexpr uint32_t W = 0x7F800000u
 template <> struct ShutGate<ElemBF16> { static constexpr uint32_t W = 0x7F807F80u; };
 template <> struct ShutGate<ElemF16> { static constexpr uint32_t W = 0x7C007C00u; };
 
-typedef RsVec<16, 1> Raw;  // 16 bytes of channels as loaded
-
-// 16 bytes of channels at p, or `fill` where the step is not part of the sequence (in = false; p
-// then points at some row that is).  PART (D is no multiple of V): a lane with fewer than V
-// channels left picks its nv elements one by one; without it every lane reads 16 bytes (lanes
-// without channels read those of channel 0: Place).
-template <class E, bool PART>
-__device__ __forceinline__ void load16(Raw& r, const typename E::T* p, int nv, bool in,
-                                       uint32_t fill) {
-  constexpr int V = E::V, S = 16 / V;
-  if (!PART || nv >= V) {
-    const RsVec<16, S> x = *reinterpret_cast<const RsVec<16, S>*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.w[i] = in ? x.w[i] : fill;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.w[i] = fill;
-    if (in) {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < nv) {
-          if (S == 4) r.w[j] = reinterpret_cast<const uint32_t*>(p)[j];
-          else {
-            const uint32_t h = reinterpret_cast<const uint16_t*>(p)[j];
-            const uint32_t old = r.w[j * S / 4];
-            r.w[j * S / 4] = (j & 1) ? (old & 0xFFFFu) | (h << 16) : (old & 0xFFFF0000u) | h;
-          }
-        }
-    }
-  }
-}
-
-template <class E>
-__device__ __forceinline__ void store16(typename E::T* p, const float* x, int nv) {
-  constexpr int V = E::V, S = 16 / V;
-  RsVec<16, S> y;
-  E::pack(x, y.w);
-  if (nv >= V) *reinterpret_cast<RsVec<16, S>*>(p) = y;
-  else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j < nv) p[j] = E::store(x[j]);
-  }
-}
-
-// V floats (a state, a gradient of one) at p
-template <int V>
-__device__ __forceinline__ void load_f(float* x, const float* p, int nv) {
-  if (nv >= V) {
-#pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      const RsVec<16, 4> r = reinterpret_cast<const RsVec<16, 4>*>(p)[q];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * q + i] = __uint_as_float(r.w[i]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = j < nv ? p[j] : 0.f;
-  }
-}
-template <int V>
-__device__ __forceinline__ void store_f(float* p, const float* x, int nv) {
-  if (nv >= V) {
-#pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      RsVec<16, 4> r;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r.w[i] = __float_as_uint(x[4 * q + i]);
-      reinterpret_cast<RsVec<16, 4>*>(p)[q] = r;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j < nv) p[j] = x[j];
-  }
-}
-
 #define REC_TINY 1e-37f  // an A that underflows stays positive: 0 would read as C = 0, "keeps all"
 
 // A and C of a run (each exact to its own last digits) as m
