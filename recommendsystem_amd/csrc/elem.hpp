@@ -22,13 +22,15 @@ struct ElemF32 {
   static constexpr int V = 4;  // elements of 16 bytes
   static __device__ __forceinline__ float load(T x) { return x; }
   static __device__ __forceinline__ T store(float x) { return x; }
+  template <int W = 4>
   static __device__ __forceinline__ void unpack(const uint32_t* w, float* x) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+    for (int i = 0; i < W; ++i) x[i] = __uint_as_float(w[i]);
   }
+  template <int W = 4>
   static __device__ __forceinline__ void pack(const float* x, uint32_t* w) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(x[i]);
+    for (int i = 0; i < W; ++i) w[i] = __float_as_uint(x[i]);
   }
 };
 
@@ -37,16 +39,18 @@ struct ElemBF16 {
   static constexpr int V = 8;
   static __device__ __forceinline__ float load(T x) { return (float)x; }
   static __device__ __forceinline__ T store(float x) { return (__bf16)x; }
+  template <int W = 4>
   static __device__ __forceinline__ void unpack(const uint32_t* w, float* x) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < W; ++i) {
       x[2 * i] = __uint_as_float(w[i] << 16);
       x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
   }
+  template <int W = 4>
   static __device__ __forceinline__ void pack(const float* x, uint32_t* w) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(pack_bf16(x[2 * i], x[2 * i + 1]));
+    for (int i = 0; i < W; ++i) w[i] = __float_as_uint(pack_bf16(x[2 * i], x[2 * i + 1]));
   }
 };
 
@@ -56,17 +60,19 @@ struct ElemF16 {
   static __device__ __forceinline__ float load(T x) { return (float)x; }
   static __device__ __forceinline__ T store(float x) { return (_Float16)x; }
   typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  template <int W = 4>
   static __device__ __forceinline__ void unpack(const uint32_t* w, float* x) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < W; ++i) {
       const f16x2 h = __builtin_bit_cast(f16x2, w[i]);
       x[2 * i] = (float)h[0];
       x[2 * i + 1] = (float)h[1];
     }
   }
+  template <int W = 4>
   static __device__ __forceinline__ void pack(const float* x, uint32_t* w) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < W; ++i) {
       const f16x2 h = {(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
       w[i] = __builtin_bit_cast(uint32_t, h);
     }

@@ -8,13 +8,11 @@
 //
 // A run of steps takes the state in front of it, s, to A s + H: A = f_1 f_2 ... is what it keeps, H
 // where it takes a zero state.  Two runs join to A = A1 A2, H = A2 H1 + H2; the gradient runs the
-// other way through the same A.  A is held as one signed number m: as A itself up to 1/2 (m > 0), as
-// -C, C = 1 - A, above (m <= 0), so that neither a long memory (A close to 1) nor a state that has
-// been forgotten (A close to 0) loses digits:  A s + H = (m <= 0 ? s : 0) + m s + H.  A workgroup owns one tile of channels and
-// walks the time axis in tiles of NG x K steps: a thread takes K consecutive steps of 16 bytes of
-// channels into registers, reduces them to (A, H), the NG runs are joined by wave shuffles and one
-// LDS exchange, and every thread then replays its own steps from the state in front of them.  So
-// everything is read once and written once, whatever the length.
+// other way through the same A.  A workgroup owns a tile of channels and walks the time axis in
+// tiles of NG x K steps: a thread takes K consecutive steps of 8 bytes of channels into registers
+// and reduces them to (A, H), the NG runs are joined by wave shuffles and one LDS exchange, and every
+// thread then replays its own steps from the state in front of them, while the next tile's loads are
+// in flight.  So everything is read once and written once, whatever the length.
 //
 // The backward computes the states again from v and g, tile by tile, from the fp32 states that
 // the forward kept in front of every tile; h itself (rounded to the rows' type) is not used.
@@ -22,9 +20,15 @@
 // Where B and D give too few workgroups to fill the chip, the time axis is cut into segments: a
 // first launch reduces every segment to its (A, H), and each workgroup of the second folds those in
 // front of its own.  The input is then read twice.
+//
+// Bound by memory; 8 bytes a lane (16 lanes to a line of 128 bytes) rather than 16 because the join
+// costs a fixed number of operations a channel and thread: twice the steps a thread, half the joins.
 #include "elem.hpp"
 
 namespace {
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 
 struct RecArgs {
   const void *v, *g, *dh;
@@ -39,13 +43,13 @@ struct RecArgs {
   void *h, *dv, *dg;
   int64_t dv_sb, dv_st, dg_sb, dg_st;
   float *last, *dh0;
-  float* ws;  // [segs][2][B D]: (m, H) of every segment
+  float* ws;  // [segs][2][B D]: (A, H) of every segment
 };
 
 template <class E>
 __device__ __forceinline__ float rec_input_gate(float g) {
   // exp = inf gives 0.  16-bit rows: the exponential's argument is rounded once, |g| half steps of fp32
-  return __builtin_amdgcn_rcpf(1.0f + (E::V == 4 ? expf(g) : __expf(g)));
+  return __builtin_amdgcn_rcpf(1.0f + (sizeof(typename E::T) == 4 ? expf(g) : __expf(g)));
 }
 
 // the bits of a gate that lets nothing in (+infinity), twice for 16-bit elements
@@ -55,22 +59,80 @@ template <> struct ShutGate<ElemF32> { static constexpr uint32_t W = 0x7F800000u
 template <> struct ShutGate<ElemBF16> { static constexpr uint32_t W = 0x7F807F80u; };
 template <> struct ShutGate<ElemF16> { static constexpr uint32_t W = 0x7C007C00u; };
 
-#define REC_TINY 1e-37f  // an A that underflows stays positive: 0 would read as C = 0, "keeps all"
+// 8 bytes of channels of a row: VC<E> elements
+template <class E>
+struct VC { static constexpr int V = 8 / (int)sizeof(typename E::T); };
+struct Half { uint32_t w[2]; };
 
-// A and C of a run (each exact to its own last digits) as m
-__device__ __forceinline__ float keep_of(float A, float C) {
-  return C < 0.5f ? -C : fmaxf(A, REC_TINY);
+// The row's channels at p (8 bytes), or `fill` where the step is not part of the sequence (in =
+// false; p then points at some row that is).  PART (D is no multiple of V): a lane with fewer than
+// V channels left picks its nv elements one by one (none for nv <= 0); without it every lane reads 8
+// bytes (lanes without channels read those of channel 0: Place).
+template <class E, bool PART>
+__device__ __forceinline__ void load8(Half& r, const typename E::T* p, int nv, bool in, uint32_t fill) {
+  constexpr int V = VC<E>::V, S = 8 / V;
+  if (!PART || nv >= V) {
+    const RsVec<8, S> x = *reinterpret_cast<const RsVec<8, S>*>(p);
+    r.w[0] = in ? x.w[0] : fill;
+    r.w[1] = in ? x.w[1] : fill;
+  } else {
+    r.w[0] = r.w[1] = fill;
+    if (in && nv > 0) {
+      if (S == 4) r.w[0] = reinterpret_cast<const uint32_t*>(p)[0];
+      else {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+        r.w[0] = (fill & 0xFFFF0000u) | h[0];
+        if (nv > 1) r.w[0] = (r.w[0] & 0xFFFFu) | ((uint32_t)h[1] << 16);
+        if (nv > 2) r.w[1] = (fill & 0xFFFF0000u) | h[2];
+      }
+    }
+  }
 }
+template <class E, bool PART>
+__device__ __forceinline__ void store8(typename E::T* p, const float* x, int nv) {
+  constexpr int V = VC<E>::V, S = 8 / V;
+  if (PART ? nv >= V : nv > 0) {
+    RsVec<8, S> y;
+    E::template pack<2>(x, y.w);
+    *reinterpret_cast<RsVec<8, S>*>(p) = y;
+  } else if (PART) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < nv) p[j] = E::store(x[j]);
+  }
+}
+// V floats (states, gradients of them)
+template <int V>
+__device__ __forceinline__ void load_n(float* x, const float* p, int nv) {
+  if (nv >= V) {
+    const RsVec<4 * V, 4> r = *reinterpret_cast<const RsVec<4 * V, 4>*>(p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = __uint_as_float(r.w[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = j < nv ? p[j] : 0.f;
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_n(float* p, const float* x, int nv) {
+  if (nv >= V) {
+    RsVec<4 * V, 4> r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) r.w[j] = __float_as_uint(x[j]);
+    *reinterpret_cast<RsVec<4 * V, 4>*>(p) = r;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < nv) p[j] = x[j];
+  }
+}
+
 // the state behind a run
-__device__ __forceinline__ float pass(float s, float m, float h) {
-  return (m <= 0.f ? s : 0.f) + fmaf(m, s, h);
-}
-// run 1, then run 2, into run 2:  A1 A2 out of A or -C on either side
-__device__ __forceinline__ void join(float m1, float h1, float& m2, float& h2) {
-  h2 = pass(h1, m2, h2);
-  const bool c1 = m1 <= 0.f, c2 = m2 <= 0.f;
-  const float p = fmaf(m1, m2, (c2 ? m1 : 0.f) + (c1 ? m2 : 0.f));
-  m2 = c1 && c2 ? (p < -0.5f ? p + 1.0f : p) : fmaxf(p, REC_TINY);
+__device__ __forceinline__ float pass(float s, float A, float h) { return fmaf(A, s, h); }
+// run 1, then run 2, into run 2
+__device__ __forceinline__ void join(float A1, float h1, float& A2, float& h2) {
+  h2 = fmaf(A2, h1, h2);
+  A2 *= A1;
 }
 
 // Which (b, channels, segment) a thread works on.
@@ -84,10 +146,10 @@ struct Place {
   __device__ __forceinline__ Place(const RecArgs& a) {
     const int tid = (int)threadIdx.x;
     if (NG == 1) {  // every thread for itself: (b, 16 bytes of channels) in one flat range
-      const int nch = (a.D + E::V - 1) / E::V;
+      const int nch = (a.D + VC<E>::V - 1) / VC<E>::V;
       const int64_t id = (int64_t)blockIdx.x * LC + tid;
       b = id / nch;
-      c0 = (int)(id % nch) * E::V;
+      c0 = (int)(id % nch) * VC<E>::V;
       nv = b < a.B ? a.D - c0 : 0;
       if (b >= a.B) b = a.B - 1;
       seg = 0;
@@ -98,7 +160,7 @@ struct Place {
       seg = a.segs > 1 ? (int)(id / per) : 0;
       id -= seg * per;
       b = id / a.nct;
-      c0 = ((int)(id % a.nct) * LC + tid % LC) * E::V;
+      c0 = ((int)(id % a.nct) * LC + tid % LC) * VC<E>::V;
       nv = a.D - c0;
       grp = tid / LC;
     }
@@ -113,7 +175,7 @@ struct Place {
 
 // Inclusive join over the groups of a wave, in time order (UP) or against it.
 template <int LC, int NG, int V, bool UP>
-__device__ __forceinline__ void wave_scan(float* C, float* H) {
+__device__ __forceinline__ void wave_scan(float* A, float* H) {
   constexpr int GW = NG == 1 ? 1 : 64 / LC;  // groups of a wave
   const int grp = (int)(threadIdx.x & 63) / LC;
 #pragma unroll
@@ -121,106 +183,181 @@ __device__ __forceinline__ void wave_scan(float* C, float* H) {
     const bool has = UP ? grp >= d : grp + d < GW;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float c1 = UP ? __shfl_up(C[j], d * LC, 64) : __shfl_down(C[j], d * LC, 64);
+      const float a1 = UP ? __shfl_up(A[j], d * LC, 64) : __shfl_down(A[j], d * LC, 64);
       const float h1 = UP ? __shfl_up(H[j], d * LC, 64) : __shfl_down(H[j], d * LC, 64);
-      if (has) join(c1, h1, C[j], H[j]);
+      if (has) join(a1, h1, A[j], H[j]);
     }
   }
 }
 
-// The state in front of this thread's run (into `in`) and, into s, behind the whole tile, from s
-// in front of the tile and the run's own (m, H); UP: in time order.  lds: [waves][2][LC * V].
+// What lies between the edge of the wave and this thread's run, onto the state at that edge.
 template <int LC, int NG, int V, bool UP>
-__device__ __forceinline__ void tile_scan(float* C, float* H, float* s, float* in, float* lds) {
+__device__ __forceinline__ void wave_inner(const float* A, const float* H, float* in) {
+  constexpr int GW = 64 / LC;
+  const int grp = (int)(threadIdx.x & 63) / LC;
+  const bool first = UP ? grp == 0 : grp == GW - 1;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float a1 = UP ? __shfl_up(A[j], LC, 64) : __shfl_down(A[j], LC, 64);
+    const float h1 = UP ? __shfl_up(H[j], LC, 64) : __shfl_down(H[j], LC, 64);
+    if (!first) in[j] = pass(in[j], a1, h1);
+  }
+}
+
+// The state at the edge of this wave's runs, into `in`, and behind the whole tile, into s, from s
+// in front of the tile and the waves' totals in lds, [waves][NT][LC * V] with the A in front: H is
+// the hi-th.  UP: in time order.
+template <int LC, int NG, int V, bool UP, int NT>
+__device__ __forceinline__ void tile_fold(const float* lds, int hi, float* s, float* in) {
+  constexpr int W = NG / (64 / LC);
+  const int lane = (int)(threadIdx.x & 63), wave = wave_id();
+#pragma unroll
+  for (int j = 0; j < V; ++j) in[j] = s[j];
+  // two waves' totals at a time: unrolled fully they would take 2 V registers a wave
+#pragma unroll 2
+  for (int k = 0; k < W; ++k) {
+    const int w = UP ? k : W - 1 - k;
+    const float* t = lds + w * NT * LC * V + (lane % LC) * V;
+    if (w == wave) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) in[j] = s[j];
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = pass(s[j], t[j], t[hi * LC * V + j]);
+  }
+}
+
+template <int LC, int NG, int V, bool UP>
+__device__ __forceinline__ bool wave_edge() {  // holds the wave's total after wave_scan
+  const int grp = (int)(threadIdx.x & 63) / LC;
+  return UP ? grp == 64 / LC - 1 : grp == 0;
+}
+
+// This wave's part of lds: the V values of a channel lane at [which][LC * V]
+template <int LC, int NG, int V, int NT>
+__device__ __forceinline__ float* wave_part(float* lds, int which) {
+  return lds + (wave_id() * NT + which) * LC * V + (int)(threadIdx.x % LC) * V;
+}
+
+// The state in front of this thread's run (into `in`) and, into s, behind the whole tile, from s
+// in front of the tile and the run's own (A, H).
+template <int LC, int NG, int V>
+__device__ __forceinline__ void tile_scan(float* A, float* H, float* s, float* in, float* lds) {
   if (NG == 1) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       in[j] = s[j];
-      s[j] = pass(s[j], C[j], H[j]);
+      s[j] = pass(s[j], A[j], H[j]);
     }
     return;
   }
-  constexpr int GW = 64 / LC, W = NG / GW;
-  const int lane = (int)(threadIdx.x & 63), grp = lane / LC, wave = wave_id();
-  wave_scan<LC, NG, V, UP>(C, H);
-  const bool edge = UP ? grp == GW - 1 : grp == 0;  // holds the wave's total
-  if (W > 1) {
-    float* mine = lds + wave * 2 * LC * V + (lane % LC) * V;
-    if (edge) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        mine[j] = C[j];
-        mine[LC * V + j] = H[j];
-      }
-    }
-    lds_barrier();
-    float sw[V];
-    // two waves' totals at a time: unrolled fully they would take 2 V registers a wave
-#pragma unroll 2
-    for (int k = 0; k < W; ++k) {
-      const int w = UP ? k : W - 1 - k;
-      const float* t = lds + w * 2 * LC * V + (lane % LC) * V;
-      if (w == wave) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) sw[j] = s[j];
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[j] = pass(s[j], t[j], t[LC * V + j]);
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) in[j] = sw[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      in[j] = s[j];
-      const int src = (UP ? 64 - LC : 0) + lane % LC;
-      s[j] = pass(s[j], __shfl(C[j], src, 64), __shfl(H[j], src, 64));
-    }
+  wave_scan<LC, NG, V, true>(A, H);
+  if (wave_edge<LC, NG, V, true>()) {
+    store_n<V>(wave_part<LC, NG, V, 2>(lds, 0), A, V);
+    store_n<V>(wave_part<LC, NG, V, 2>(lds, 1), H, V);
   }
-  // what lies between the wave's edge and this thread's run
-  const bool first = UP ? grp == 0 : grp == GW - 1;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float c1 = UP ? __shfl_up(C[j], LC, 64) : __shfl_down(C[j], LC, 64);
-    const float h1 = UP ? __shfl_up(H[j], LC, 64) : __shfl_down(H[j], LC, 64);
-    if (!first) in[j] = pass(in[j], c1, h1);
-  }
+  lds_barrier();
+  tile_fold<LC, NG, V, true, 2>(lds, 1, s, in);
+  wave_inner<LC, NG, V, true>(A, H, in);
 }
 
-// The (m, H) of all of the workgroup's runs in order, in every thread.  lds as in tile_scan.
-template <int LC, int NG, int V, bool UP>
-__device__ __forceinline__ void tile_total(float* C, float* H, float* lds) {
-  constexpr int GW = 64 / LC, W = NG / GW;
-  const int lane = (int)(threadIdx.x & 63), grp = lane / LC, wave = wave_id();
-  wave_scan<LC, NG, V, UP>(C, H);
-  float* mine = lds + wave * 2 * LC * V + (lane % LC) * V;
-  if (UP ? grp == GW - 1 : grp == 0) {
+// Both directions at once, behind one barrier: (A, H) from s in time order and (A, G) from r
+// against it.
+template <int LC, int NG, int V>
+__device__ __forceinline__ void tile_scan_both(float* A, float* H, float* G, float* s, float* r,
+                                               float* in_s, float* in_r, float* lds) {
+  if (NG == 1) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      mine[j] = C[j];
-      mine[LC * V + j] = H[j];
+      in_s[j] = s[j];
+      in_r[j] = r[j];
+      r[j] = pass(r[j], A[j], G[j]);
     }
+    return;
+  }
+  float A2[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) A2[j] = A[j];
+  wave_scan<LC, NG, V, true>(A, H);
+  wave_scan<LC, NG, V, false>(A2, G);
+  if (wave_edge<LC, NG, V, true>()) {
+    store_n<V>(wave_part<LC, NG, V, 3>(lds, 0), A, V);
+    store_n<V>(wave_part<LC, NG, V, 3>(lds, 1), H, V);
+  }
+  if (wave_edge<LC, NG, V, false>()) store_n<V>(wave_part<LC, NG, V, 3>(lds, 2), G, V);
+  lds_barrier();
+  tile_fold<LC, NG, V, true, 3>(lds, 1, s, in_s);
+  tile_fold<LC, NG, V, false, 3>(lds, 2, r, in_r);
+  wave_inner<LC, NG, V, true>(A, H, in_s);
+  wave_inner<LC, NG, V, false>(A2, G, in_r);
+}
+
+// The (A, H) of all of the workgroup's runs in order, in every thread.
+template <int LC, int NG, int V, bool UP>
+__device__ __forceinline__ void tile_total(float* A, float* H, float* lds) {
+  constexpr int W = NG / (64 / LC);
+  wave_scan<LC, NG, V, UP>(A, H);
+  if (wave_edge<LC, NG, V, UP>()) {
+    store_n<V>(wave_part<LC, NG, V, 2>(lds, 0), A, V);
+    store_n<V>(wave_part<LC, NG, V, 2>(lds, 1), H, V);
   }
   lds_barrier();
 #pragma unroll
-  for (int j = 0; j < V; ++j) C[j] = H[j] = 0.f;
+  for (int j = 0; j < V; ++j) {
+    A[j] = 1.f;
+    H[j] = 0.f;
+  }
 #pragma unroll 2
   for (int k = 0; k < W; ++k) {
-    const float* t = lds + (UP ? k : W - 1 - k) * 2 * LC * V + (lane % LC) * V;
+    const float* t = lds + (UP ? k : W - 1 - k) * 2 * LC * V + (int)(threadIdx.x % LC) * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float c = t[j], h = t[LC * V + j];
-      join(C[j], H[j], c, h);
-      C[j] = c;
-      H[j] = h;
+      float a2 = t[j], h2 = t[LC * V + j];
+      join(A[j], H[j], a2, h2);
+      A[j] = a2;
+      H[j] = h2;
     }
   }
 }
 
-template <int LC, int NG, int V>
-struct ScanLds {  // two buffers: one barrier a tile is enough
-  static constexpr int W = NG == 1 ? 1 : NG / (64 / LC);
-  static constexpr int FLOATS = W * 2 * LC * V;
+// One [B, T, D] array as a thread reads or writes it: its K steps of every tile.  The workgroup's
+// sequence and a wave's first step are the same in all lanes, so addresses are a scalar base and one
+// 32-bit offset a lane (rec_strides_ok bounds the strides); only where every thread works for itself
+// (NG == 1) they are 64-bit a lane.
+template <class E, int LC, int NG, int K, class Ptr>
+struct Rows {
+  typedef typename E::T X;
+  Ptr base;
+  int64_t st;
+  uint32_t off;  // of the lane's first step and channel
+  int c, ls;     // its channel; its first step of the wave's
+  __device__ __forceinline__ Rows(Ptr p, int64_t b, int64_t sb, int64_t st_, int c_) : st(st_), c(c_) {
+    ls = NG == 1 ? 0 : (int)(threadIdx.x & 63) / LC * K;
+    base = NG == 1 ? p + b * sb + c : p + b * sb;
+    off = NG == 1 ? 0u : (uint32_t)ls * (uint32_t)st + (uint32_t)c;
+  }
+  // step k of the thread; t: the wave's first step (NG == 1: the thread's)
+  __device__ __forceinline__ Ptr at(int64_t t, int k) const { return base + (t + k) * st + off; }
+  // the same within 0 .. n - 1 (n >= 1)
+  __device__ __forceinline__ Ptr in(int64_t t, int k, int64_t n) const {
+    const int64_t tb = t < n - 1 ? t : n - 1;
+    if (NG == 1) return base + (t + k < n ? t + k : n - 1) * st;
+    const int64_t most = n - 1 - tb;
+    const uint32_t d = (uint32_t)(ls + k < most ? ls + k : most);
+    return base + tb * st + (d * (uint32_t)st + (uint32_t)c);
+  }
+};
+// the first step of a wave (NG == 1: of a thread) in a tile
+template <int LC, int NG, int K>
+__device__ __forceinline__ int64_t wave_step(int tile) {
+  return NG == 1 ? (int64_t)tile * K : (int64_t)tile * (NG * K) + wave_id() * (64 / LC) * K;
+}
+
+// floats of NT values a channel and wave; kernels that join tile after tile use two in turn, so that
+// one barrier a tile is enough
+template <int LC, int NG, int V, int NT>
+struct ScanLds {
+  static constexpr int FLOATS = NG == 1 ? 1 : NG / (64 / LC) * NT * LC * V;
 };
 
 }  // namespace
@@ -230,92 +367,99 @@ struct ScanLds {  // two buffers: one barrier a tile is enough
 // ---------------------------------------------------------------------------------------------
 template <class E, int LC, int NG, int K, bool PART>
 __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
-  constexpr int V = E::V, STEPS = NG * K;
+  constexpr int V = VC<E>::V, STEPS = NG * K;
   typedef typename E::T X;
-  __shared__ __attribute__((aligned(16))) float lds[2][ScanLds<LC, NG, V>::FLOATS];
+  __shared__ __attribute__((aligned(16))) float lds[2][ScanLds<LC, NG, V, 2>::FLOATS];
   const Place<E, LC, NG> p(a);
-  const X* vp = (const X*)a.v + p.b * a.v_sb + p.cl;
-  const X* gp = (const X*)a.g + p.b * a.g_sb + p.cl;
-  X* hp = (X*)a.h + p.b * a.T * a.D + p.c0;
+  typedef Rows<E, LC, NG, K, const X*> In;
+  const In rv_((const X*)a.v, p.b, a.v_sb, a.v_st, p.cl), rg_((const X*)a.g, p.b, a.g_sb, a.g_st, p.cl);
+  const Rows<E, LC, NG, K, X*> rh_((X*)a.h, p.b, a.T * a.D, a.D, p.c0);
+  const int64_t some = p.n > 0 ? p.n : 1;  // steps that may be read
   const int64_t ch = p.b * a.D + p.c0;
   const int t0 = p.seg * a.tps, t1 = min(a.tiles, t0 + a.tps);
 
   float s[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = 0.f;
-  if (a.h0) load_f<V>(s, a.h0 + ch, p.nv);
+  if (a.h0) load_n<V>(s, a.h0 + ch, p.nv);
   for (int k = 0; k < p.seg; ++k) {
-    float C[V], H[V];
+    float A[V], H[V];
     const float* w = a.ws + (int64_t)k * 2 * a.B * a.D + ch;
-    load_f<V>(C, w, p.nv);
-    load_f<V>(H, w + a.B * a.D, p.nv);
+    load_n<V>(A, w, p.nv);
+    load_n<V>(H, w + a.B * a.D, p.nv);
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = pass(s[j], C[j], H[j]);
+    for (int j = 0; j < V; ++j) s[j] = pass(s[j], A[j], H[j]);
   }
 
-  Raw nv_[K], ng_[K];
-  auto load = [&](int tile) {
-    const int64_t t = (int64_t)tile * STEPS + p.grp * K;
-    const X *vt = vp + t * a.v_st, *gt = gp + t * a.g_st;
+  Half nv_[K], ng_[K];
+  // (whole: every step of the tile is part of the sequence)
+  auto load_as = [&](int tile, auto whole) __attribute__((always_inline)) {
+    const int64_t t = wave_step<LC, NG, K>(tile);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const bool in = t + k < p.n;
-      load16<E, PART>(nv_[k], in ? vt + k * a.v_st : vp, p.nv, in, 0u);
-      load16<E, PART>(ng_[k], in ? gt + k * a.g_st : gp, p.nv, in, ShutGate<E>::W);
+      constexpr bool W = decltype(whole)::value;
+      const bool in = W || t + rv_.ls + k < p.n;
+      load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, some), p.nv, in, 0u);
+      load8<E, PART>(ng_[k], W ? rg_.at(t, k) : rg_.in(t, k, some), p.nv, in, ShutGate<E>::W);
     }
+  };
+  auto load = [&](int tile) __attribute__((always_inline)) {
+    if (NG > 1 && (int64_t)(tile + 1) * STEPS <= p.n) load_as(tile, Yes());
+    else load_as(tile, No());
   };
   if (t1 > t0) load(t0);
   for (int tile = t0; tile < t1; ++tile) {
-    Raw rv[K];
-    float in[K][V], A[V], C[V], H[V], st[V];
+    Half rv[K];
+    float in[K][V], A[V], H[V], st[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       A[j] = 1.f;
-      C[j] = H[j] = 0.f;
+      H[j] = 0.f;
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float g[V], v[V];
       rv[k] = nv_[k];
-      E::unpack(ng_[k].w, g);
-      E::unpack(rv[k].w, v);
+      E::template unpack<2>(ng_[k].w, g);
+      E::template unpack<2>(rv[k].w, v);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float i = in[k][j] = rec_input_gate<E>(g[j]);
         H[j] = fmaf(i, v[j] - H[j], H[j]);
         A[j] = fmaf(-i, A[j], A[j]);
-        C[j] = fmaf(i, 1.0f - C[j], C[j]);
       }
     }
     if (tile + 1 < t1) load(tile + 1);
     if (a.states && p.grp == 0)
-      store_f<V>(a.states + (p.b * a.tiles + tile) * a.D + p.c0, s, p.nv);
+      store_n<V>(a.states + (p.b * a.tiles + tile) * a.D + p.c0, s, p.nv);
+    tile_scan<LC, NG, V>(A, H, s, st, lds[tile & 1]);
+    auto replay = [&](auto whole) __attribute__((always_inline)) {
+      const int64_t t = wave_step<LC, NG, K>(tile);
 #pragma unroll
-    for (int j = 0; j < V; ++j) C[j] = keep_of(A[j], C[j]);
-    tile_scan<LC, NG, V, true>(C, H, s, st, lds[tile & 1]);
+      for (int k = 0; k < K; ++k) {
+        float v[V], o[V];
+        E::template unpack<2>(rv[k].w, v);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t t = (int64_t)tile * STEPS + p.grp * K + k;
-      float v[V], o[V];
-      E::unpack(rv[k].w, v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        st[j] = fmaf(in[k][j], v[j] - st[j], st[j]);
-        o[j] = t < p.n ? st[j] : 0.f;
+        for (int j = 0; j < V; ++j) {
+          st[j] = fmaf(in[k][j], v[j] - st[j], st[j]);
+          o[j] = decltype(whole)::value || t + rh_.ls + k < p.n ? st[j] : 0.f;
+        }
+        if (decltype(whole)::value || t + rh_.ls + k < a.T) store8<E, PART>(rh_.at(t, k), o, p.nv);
       }
-      if (t < a.T) store16<E>(hp + t * a.D, o, p.nv);
-    }
+    };
+    if (NG > 1 && (int64_t)(tile + 1) * STEPS <= p.n) replay(Yes());
+    else replay(No());
   }
-  if (p.grp == 0 && t1 == a.tiles) store_f<V>(a.last + ch, s, p.nv);
+  if (p.grp == 0 && t1 == a.tiles) store_n<V>(a.last + ch, s, p.nv);
 }
 
 // (A, H) of every segment but the last (backward: of every one but the first, over dh, against
 // time).  A group takes one run of consecutive steps of the segment, so the runs are joined once.
 template <class E, int LC, int NG, int K, bool FWD, bool PART>
 __global__ void __launch_bounds__(LC * NG) rec_sum_kernel(const RecArgs a) {
-  constexpr int V = E::V, STEPS = NG * K;
+  constexpr int V = VC<E>::V, STEPS = NG * K;
   typedef typename E::T X;
-  __shared__ __attribute__((aligned(16))) float lds[ScanLds<LC, NG, V>::FLOATS];
+  __shared__ __attribute__((aligned(16))) float lds[ScanLds<LC, NG, V, 2>::FLOATS];
   Place<E, LC, NG> p(a);
   if (!FWD) p.seg += 1;
   // (no dh: the gates' rows are read in its place, and not used)
@@ -325,47 +469,43 @@ __global__ void __launch_bounds__(LC * NG) rec_sum_kernel(const RecArgs a) {
                     : none ? gp : (const X*)a.dh + p.b * a.dh_sb + p.cl;
   const int64_t x_st = FWD ? a.v_st : none ? a.g_st : a.dh_st;
   const int run = a.tps * K;  // steps of a group
+  const bool whole = (int64_t)(p.seg + 1) * a.tps * STEPS <= p.n;
   const int64_t first = (int64_t)p.seg * a.tps * STEPS + (int64_t)p.grp * run;
-  float A[V], C[V], H[V];
+  float A[V], H[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     A[j] = 1.f;
-    C[j] = H[j] = 0.f;
+    H[j] = 0.f;
   }
   for (int q = 0; q < a.tps; ++q) {
-    Raw rx[K], rg[K];
+    Half rx[K], rg[K];
     const int64_t t = first + (FWD ? q * K : run - 1 - q * K);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      {
-        const int64_t tk = FWD ? t + k : t - k;
-        const bool in = tk < p.n;
-        load16<E, PART>(rx[k], in ? xp + tk * x_st : xp, p.nv, in && !none, 0u);
-        load16<E, PART>(rg[k], in ? gp + tk * a.g_st : gp, p.nv, in, ShutGate<E>::W);
-      }
+      const int64_t tk = FWD ? t + k : t - k;
+      const bool in = whole || tk < p.n;
+      load8<E, PART>(rx[k], in ? xp + tk * x_st : xp, p.nv, in && !none, 0u);
+      load8<E, PART>(rg[k], in ? gp + tk * a.g_st : gp, p.nv, in, ShutGate<E>::W);
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float g[V], x[V];
-      E::unpack(rg[k].w, g);
-      E::unpack(rx[k].w, x);
+      E::template unpack<2>(rg[k].w, g);
+      E::template unpack<2>(rx[k].w, x);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float i = rec_input_gate<E>(g[j]);
         if (FWD) H[j] = fmaf(i, x[j] - H[j], H[j]);
         else H[j] = fmaf(-i, x[j] + H[j], x[j] + H[j]);
         A[j] = fmaf(-i, A[j], A[j]);
-        C[j] = fmaf(i, 1.0f - C[j], C[j]);
       }
     }
   }
-#pragma unroll
-  for (int j = 0; j < V; ++j) C[j] = keep_of(A[j], C[j]);
-  tile_total<LC, NG, V, FWD>(C, H, lds);
+  tile_total<LC, NG, V, FWD>(A, H, lds);
   if (p.grp == 0) {
     float* w = a.ws + (int64_t)p.seg * 2 * a.B * a.D + p.b * a.D + p.c0;
-    store_f<V>(w, C, p.nv);
-    store_f<V>(w + a.B * a.D, H, p.nv);
+    store_n<V>(w, A, p.nv);
+    store_n<V>(w + a.B * a.D, H, p.nv);
   }
 }
 
@@ -374,76 +514,79 @@ __global__ void __launch_bounds__(LC * NG) rec_sum_kernel(const RecArgs a) {
 // ---------------------------------------------------------------------------------------------
 template <class E, int LC, int NG, int K, bool PART>
 __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
-  constexpr int V = E::V, STEPS = NG * K;
+  constexpr int V = VC<E>::V, STEPS = NG * K;
   typedef typename E::T X;
-  __shared__ __attribute__((aligned(16))) float lds[2][2][ScanLds<LC, NG, V>::FLOATS];
+  __shared__ __attribute__((aligned(16))) float lds[2][ScanLds<LC, NG, V, 3>::FLOATS];
   const Place<E, LC, NG> p(a);
-  const X* vp = (const X*)a.v + p.b * a.v_sb + p.cl;
-  const X* gp = (const X*)a.g + p.b * a.g_sb + p.cl;
+  typedef Rows<E, LC, NG, K, const X*> In;
+  typedef Rows<E, LC, NG, K, X*> Out;
   // (no dh: the gates' rows are read in its place, and not used)
   const bool none = !a.dh;
-  const X* dp = none ? gp : (const X*)a.dh + p.b * a.dh_sb + p.cl;
-  const int64_t d_st = none ? a.g_st : a.dh_st;
-  X* dvp = (X*)a.dv + p.b * a.dv_sb + p.c0;
-  X* dgp = (X*)a.dg + p.b * a.dg_sb + p.c0;
+  const In rv_((const X*)a.v, p.b, a.v_sb, a.v_st, p.cl), rg_((const X*)a.g, p.b, a.g_sb, a.g_st, p.cl),
+      rd_((const X*)(none ? a.g : a.dh), p.b, none ? a.g_sb : a.dh_sb, none ? a.g_st : a.dh_st, p.cl);
+  const Out rdv_((X*)a.dv, p.b, a.dv_sb, a.dv_st, p.c0), rdg_((X*)a.dg, p.b, a.dg_sb, a.dg_st, p.c0);
+  const int64_t some = p.n > 0 ? p.n : 1;  // steps that may be read
   const int64_t ch = p.b * a.D + p.c0;
   const int t0 = p.seg * a.tps, t1 = min(a.tiles, t0 + a.tps);
 
   float r[V];  // the gradient from behind the tile
 #pragma unroll
   for (int j = 0; j < V; ++j) r[j] = 0.f;
-  if (a.dlast) load_f<V>(r, a.dlast + ch, p.nv);
+  if (a.dlast) load_n<V>(r, a.dlast + ch, p.nv);
   for (int k = a.segs - 1; k > p.seg; --k) {
-    float C[V], G[V];
+    float A[V], G[V];
     const float* w = a.ws + (int64_t)k * 2 * a.B * a.D + ch;
-    load_f<V>(C, w, p.nv);
-    load_f<V>(G, w + a.B * a.D, p.nv);
+    load_n<V>(A, w, p.nv);
+    load_n<V>(G, w + a.B * a.D, p.nv);
 #pragma unroll
-    for (int j = 0; j < V; ++j) r[j] = pass(r[j], C[j], G[j]);
+    for (int j = 0; j < V; ++j) r[j] = pass(r[j], A[j], G[j]);
   }
 
-  Raw nv_[K], ng_[K], nd_[K];
+  Half nv_[K], ng_[K], nd_[K];
   float ns[V];
-  auto load = [&](int tile) {
-    const int64_t t = (int64_t)tile * STEPS + p.grp * K;
-    const X *vt = vp + t * a.v_st, *gt = gp + t * a.g_st, *dt = dp + t * d_st;
+  auto load_as = [&](int tile, auto whole) __attribute__((always_inline)) {
+    const int64_t t = wave_step<LC, NG, K>(tile);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const bool in = t + k < p.n;
-      load16<E, PART>(ng_[k], in ? gt + k * a.g_st : gp, p.nv, in, ShutGate<E>::W);
-      load16<E, PART>(nv_[k], in ? vt + k * a.v_st : vp, p.nv, in, 0u);
-      load16<E, PART>(nd_[k], in ? dt + k * d_st : dp, p.nv, in && !none, 0u);
+      constexpr bool W = decltype(whole)::value;
+      const bool in = W || t + rv_.ls + k < p.n;
+      load8<E, PART>(ng_[k], W ? rg_.at(t, k) : rg_.in(t, k, some), p.nv, in, ShutGate<E>::W);
+      load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, some), p.nv, in, 0u);
+      load8<E, PART>(nd_[k], W ? rd_.at(t, k) : rd_.in(t, k, some), p.nv, in && !none, 0u);
     }
-    load_f<V>(ns, a.states + (p.b * a.tiles + tile) * a.D + p.c0, p.nv);
+    load_n<V>(ns, a.states + (p.b * a.tiles + tile) * a.D + p.c0, p.nv);
+  };
+  auto load = [&](int tile) __attribute__((always_inline)) {
+    if (NG > 1 && (int64_t)(tile + 1) * STEPS <= p.n) load_as(tile, Yes());
+    else load_as(tile, No());
   };
   if (t1 > t0) load(t1 - 1);
   for (int tile = t1 - 1; tile >= t0; --tile) {
-    Raw rd[K];
-    float in[K][V], e[K][V], A[V], C[V], H[V], G[V], s[V], st[V], rt[V];
+    Half rd[K];
+    float in[K][V], e[K][V], A[V], H[V], G[V], s[V], st[V], rt[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       A[j] = 1.f;
-      C[j] = H[j] = G[j] = 0.f;
+      H[j] = G[j] = 0.f;
       s[j] = ns[j];
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float g[V];
       rd[k] = nd_[k];
-      E::unpack(ng_[k].w, g);
-      E::unpack(nv_[k].w, e[k]);
+      E::template unpack<2>(ng_[k].w, g);
+      E::template unpack<2>(nv_[k].w, e[k]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float i = in[k][j] = rec_input_gate<E>(g[j]);
         H[j] = fmaf(i, e[k][j] - H[j], H[j]);
         A[j] = fmaf(-i, A[j], A[j]);
-        C[j] = fmaf(i, 1.0f - C[j], C[j]);
       }
     }
 #pragma unroll
     for (int k = K - 1; k >= 0; --k) {
       float d[V];
-      E::unpack(rd[k].w, d);
+      E::template unpack<2>(rd[k].w, d);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float x = d[j] + G[j];
@@ -451,11 +594,7 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
       }
     }
     if (tile > t0) load(tile - 1);
-    float C2[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) C2[j] = C[j] = keep_of(A[j], C[j]);
-    tile_scan<LC, NG, V, true>(C, H, s, st, lds[tile & 1][0]);
-    tile_scan<LC, NG, V, false>(C2, G, r, rt, lds[tile & 1][1]);
+    tile_scan_both<LC, NG, V>(A, H, G, s, r, st, rt, lds[tile & 1]);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -466,9 +605,9 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
       }
 #pragma unroll
     for (int k = K - 1; k >= 0; --k) {
-      const int64_t t = (int64_t)tile * STEPS + p.grp * K + k;
+      const int64_t t = wave_step<LC, NG, K>(tile);
       float d[V], gv[V], gg[V];
-      E::unpack(rd[k].w, d);
+      E::template unpack<2>(rd[k].w, d);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float i = in[k][j], x = d[j] + rt[j];
@@ -476,13 +615,13 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
         gg[j] = gv[j] * e[k][j] * (1.0f - i);
         rt[j] = x - gv[j];
       }
-      if (t < a.T) {
-        store16<E>(dvp + t * a.dv_st, gv, p.nv);
-        store16<E>(dgp + t * a.dg_st, gg, p.nv);
+      if (t + rdv_.ls + k < a.T) {
+        store8<E, PART>(rdv_.at(t, k), gv, p.nv);
+        store8<E, PART>(rdg_.at(t, k), gg, p.nv);
       }
     }
   }
-  if (p.grp == 0 && t0 == 0 && a.dh0) store_f<V>(a.dh0 + ch, r, p.nv);
+  if (p.grp == 0 && t0 == 0 && a.dh0) store_n<V>(a.dh0 + ch, r, p.nv);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -490,7 +629,7 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
 // ---------------------------------------------------------------------------------------------
 template <class E>
 __global__ void __launch_bounds__(256) rec_step_kernel(const RecArgs a, float* new_state) {
-  constexpr int V = E::V;
+  constexpr int V = VC<E>::V;
   typedef typename E::T X;
   const int nch = (a.D + V - 1) / V;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -498,18 +637,18 @@ __global__ void __launch_bounds__(256) rec_step_kernel(const RecArgs a, float* n
   const int64_t b = id / nch;
   const int c0 = (int)(id % nch) * V, nv = a.D - c0;
   float s[V], v[V], g[V];
-  Raw rv, rg;
-  load16<E, true>(rv, (const X*)a.v + b * a.v_sb + c0, nv, true, 0u);
-  load16<E, true>(rg, (const X*)a.g + b * a.g_sb + c0, nv, true, 0u);
+  Half rv, rg;
+  load8<E, true>(rv, (const X*)a.v + b * a.v_sb + c0, nv, true, 0u);
+  load8<E, true>(rg, (const X*)a.g + b * a.g_sb + c0, nv, true, 0u);
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = 0.f;
-  if (a.h0) load_f<V>(s, a.h0 + b * a.D + c0, nv);
-  E::unpack(rv.w, v);
-  E::unpack(rg.w, g);
+  if (a.h0) load_n<V>(s, a.h0 + b * a.D + c0, nv);
+  E::template unpack<2>(rv.w, v);
+  E::template unpack<2>(rg.w, g);
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = fmaf(rec_input_gate<E>(g[j]), v[j] - s[j], s[j]);
-  store16<E>((X*)a.h + b * a.D + c0, s, nv);
-  store_f<V>(new_state + b * a.D + c0, s, nv);
+  store8<E, true>((X*)a.h + b * a.D + c0, s, nv);
+  store_n<V>(new_state + b * a.D + c0, s, nv);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -518,6 +657,7 @@ __global__ void __launch_bounds__(256) rec_step_kernel(const RecArgs a, float* n
 // ---------------------------------------------------------------------------------------------
 namespace {
 
+constexpr int REC_LC = 16;  // lanes to a row of a channel tile: 128 bytes
 enum { REC_FLAT, REC_WAVE, REC_BLOCK };
 struct RecPlan {
   int kind, steps;  // steps: of a time tile
@@ -526,9 +666,9 @@ struct RecPlan {
 };
 
 RecPlan rec_plan(int dtype, int64_t B, int64_t T, int D) {
-  const int V = dtype == RS_F32 ? 4 : 8;
+  const int V = dtype == RS_F32 ? 2 : 4;
   RecPlan p;
-  p.nct = (D + 8 * V - 1) / (8 * V);
+  p.nct = (D + REC_LC * V - 1) / (REC_LC * V);
   const int64_t blocks = B * p.nct;
   p.kind = T <= 8 ? REC_FLAT : T <= 64 || blocks >= 2048 ? REC_WAVE : REC_BLOCK;
   p.steps = p.kind == REC_FLAT ? 8 : p.kind == REC_WAVE ? 64 : 256;
@@ -557,13 +697,13 @@ template <class E, bool PART>
 int rec_fwd_as(hipStream_t s, const RecPlan& p, const RecArgs& a) {
   const unsigned per = (unsigned)(a.B * a.nct);
   if (p.kind == REC_FLAT) {
-    const int64_t n = a.B * ((a.D + E::V - 1) / E::V);
+    const int64_t n = a.B * ((a.D + VC<E>::V - 1) / VC<E>::V);
     rec_fwd_kernel<E, 64, 1, 8, PART><<<(unsigned)((n + 63) / 64), 64, 0, s>>>(a);
   } else if (p.kind == REC_WAVE) {
-    rec_fwd_kernel<E, 8, 8, 8, PART><<<per, 64, 0, s>>>(a);
+    rec_fwd_kernel<E, REC_LC, 8, 8, PART><<<per, 128, 0, s>>>(a);
   } else {
-    if (p.segs > 1) rec_sum_kernel<E, 8, 32, 8, true, PART><<<per * (p.segs - 1), 256, 0, s>>>(a);
-    rec_fwd_kernel<E, 8, 32, 8, PART><<<per * p.segs, 256, 0, s>>>(a);
+    if (p.segs > 1) rec_sum_kernel<E, REC_LC, 16, 16, true, PART><<<per * (p.segs - 1), 256, 0, s>>>(a);
+    rec_fwd_kernel<E, REC_LC, 32, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
   }
   return rs_status_after_launch();
 }
@@ -572,31 +712,36 @@ template <class E, bool PART>
 int rec_bwd_as(hipStream_t s, const RecPlan& p, const RecArgs& a) {
   const unsigned per = (unsigned)(a.B * a.nct);
   if (p.kind == REC_FLAT) {
-    const int64_t n = a.B * ((a.D + E::V - 1) / E::V);
+    const int64_t n = a.B * ((a.D + VC<E>::V - 1) / VC<E>::V);
     rec_bwd_kernel<E, 64, 1, 8, PART><<<(unsigned)((n + 63) / 64), 64, 0, s>>>(a);
   } else if (p.kind == REC_WAVE) {
-    rec_bwd_kernel<E, 8, 16, 4, PART><<<per, 128, 0, s>>>(a);
+    rec_bwd_kernel<E, REC_LC, 8, 8, PART><<<per, 128, 0, s>>>(a);
   } else {
-    if (p.segs > 1) rec_sum_kernel<E, 8, 32, 8, false, PART><<<per * (p.segs - 1), 256, 0, s>>>(a);
-    rec_bwd_kernel<E, 8, 64, 4, PART><<<per * p.segs, 512, 0, s>>>(a);
+    if (p.segs > 1) rec_sum_kernel<E, REC_LC, 16, 16, false, PART><<<per * (p.segs - 1), 256, 0, s>>>(a);
+    rec_bwd_kernel<E, REC_LC, 32, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
   }
   return rs_status_after_launch();
 }
 
 template <class E>
 int rec_fwd(hipStream_t s, const RecPlan& p, const RecArgs& a) {
-  return a.D % E::V ? rec_fwd_as<E, true>(s, p, a) : rec_fwd_as<E, false>(s, p, a);
+  return a.D % VC<E>::V ? rec_fwd_as<E, true>(s, p, a) : rec_fwd_as<E, false>(s, p, a);
 }
 template <class E>
 int rec_bwd(hipStream_t s, const RecPlan& p, const RecArgs& a) {
-  return a.D % E::V ? rec_bwd_as<E, true>(s, p, a) : rec_bwd_as<E, false>(s, p, a);
+  return a.D % VC<E>::V ? rec_bwd_as<E, true>(s, p, a) : rec_bwd_as<E, false>(s, p, a);
 }
 
 template <class E>
 int rec_step(hipStream_t s, const RecArgs& a, float* new_state) {
-  const int64_t n = a.B * ((a.D + E::V - 1) / E::V);
+  const int64_t n = a.B * ((a.D + VC<E>::V - 1) / VC<E>::V);
   rec_step_kernel<E><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, new_state);
   return rs_status_after_launch();
+}
+
+// a wave's 64 steps of 2^23 elements of 4 bytes: 2^31 bytes, which a lane's offset holds
+bool rec_strides_ok(int64_t a, int64_t b, int64_t c) {
+  return a < (1 << 23) && b < (1 << 23) && c < (1 << 23);
 }
 
 // what the launches index: workgroups and time tiles in 31 bits
@@ -626,6 +771,7 @@ RS_API int rs_gated_rec_fwd(void* stream, int dtype, const void* v, int64_t v_sb
   if (B == 0) return RS_OK;
   if (!last || (T > 0 && (!v || !g || !h || v_sb < 0 || v_st < 0 || g_sb < 0 || g_st < 0)))
     return RS_ERR_ARG;
+  if (!rec_strides_ok(v_st, g_st, D)) return RS_ERR_UNSUPPORTED;
   const int64_t need = rs_gated_rec_workspace_floats(dtype, B, T, D);
   if (need > 0 && (!workspace || workspace_floats < need)) return RS_ERR_ARG;
   const RecPlan p = rec_plan(dtype, B, T, D);
@@ -650,6 +796,7 @@ RS_API int rs_gated_rec_bwd(void* stream, int dtype, const void* v, int64_t v_sb
                 (B > 1 && (dv_sb < D || dg_sb < D))))
     return RS_ERR_ARG;
   if (T == 0 && !dh0) return RS_OK;
+  if (!rec_strides_ok(v_st, g_st, dh_st) || !rec_strides_ok(dv_st, dg_st, D)) return RS_ERR_UNSUPPORTED;
   const int64_t need = rs_gated_rec_workspace_floats(dtype, B, T, D);
   if (need > 0 && (!workspace || workspace_floats < need)) return RS_ERR_ARG;
   const RecPlan p = rec_plan(dtype, B, T, D);

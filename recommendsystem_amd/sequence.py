@@ -160,9 +160,14 @@ class LayerNormalization(nn.Module):
 # ============================================================================================
 # gated linear recurrence
 # ============================================================================================
+MAX_STEP_STRIDE = 2 ** 23  # elements between two steps (and of a step) that the kernels index
+
+
 def _unit(t):
-    """t [B, T, D] with unit stride along D and no negative strides, in place where possible."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """t [B, T, D] or [B, D] as the kernels read it: in place with unit stride along D and steps
+    not too far apart, a contiguous copy otherwise."""
+    unit = t.stride(-1) == 1 or t.shape[-1] == 1
+    return t if unit and (t.dim() < 3 or t.stride(1) < MAX_STEP_STRIDE) else t.contiguous()
 
 
 def _halves(v, g):
@@ -188,6 +193,8 @@ def _check_rec(v, g, dims, what):
             raise ValueError(f"{what}: values {tuple(v.shape)} and gates {tuple(g.shape)} differ in shape")
         if v.shape[-1] < 1:
             raise ValueError(f"{what} needs a last dimension of at least 1, got shape {tuple(v.shape)}")
+    if v.shape[-1] >= MAX_STEP_STRIDE:
+        raise ValueError(f"{what}: a last dimension of {v.shape[-1]} is not supported")
     return code
 
 

@@ -521,14 +521,16 @@ def test_offsets_past_32_bits():
     assert torch.equal(unpack8(codes, scales, torch.bfloat16)[-9:], unpack8(ct, st, torch.bfloat16))
     del codes, scales
     # one history of 2^21 events; gates around 0 forget within some tens of steps
-    v = x.view(1, R, D).requires_grad_()
-    h, last = gated_recurrence(v, v)
-    dv, = torch.autograd.grad((h, last), v, (v.detach(), torch.ones_like(last)))
-    tv = v.detach()[:, -400:].clone().requires_grad_()
-    th, tlast = gated_recurrence(tv, tv)
-    tdv, = torch.autograd.grad((th, tlast), tv, (tv.detach(), torch.ones_like(tlast)))
+    # (values and gates are two leaves of one memory: summed, their gradients would be rounded to
+    # the type once more, and cancel)
+    v, g = x.view(1, R, D).requires_grad_(), x.view(1, R, D).detach().requires_grad_()
+    h, last = gated_recurrence(v, g)
+    dv, dg = torch.autograd.grad((h, last), (v, g), (v.detach(), torch.ones_like(last)))
+    tv, tg = (t.detach()[:, -400:].clone().requires_grad_() for t in (v, g))
+    th, tlast = gated_recurrence(tv, tg)
+    tdv, tdg = torch.autograd.grad((th, tlast), (tv, tg), (tv.detach(), torch.ones_like(tlast)))
     # fp32 values that differ in their last digits round to neighbours: one step of the type
-    for a, b in ((h[:, -200:], th[:, -200:]), (dv[:, -200:], tdv[:, -200:])):
+    for a, b in ((h[:, -200:], th[:, -200:]), (dv[:, -200:], tdv[:, -200:]), (dg[:, -200:], tdg[:, -200:])):
         assert bool(((a.float() - b.float()).abs() <= 2 * 2.0 ** -8 * b.float().abs() + 1e-5).all())
     near(last, tlast.double().cpu(), 64 * U * (1 + tlast.double().cpu().abs()), "last")
 
