@@ -135,6 +135,15 @@ __device__ __forceinline__ void join(float A1, float h1, float& A2, float& h2) {
   A2 *= A1;
 }
 
+// Workgroups are dealt out to the 8 XCDs in turn, each with an L2 of its own.  Numbering them so that
+// an XCD gets a run of consecutive ones puts the channel tiles of a row side by side: where rows do
+// not start on lines of 128 bytes, neighbours share a line, which two XCDs would both fetch
+// (65521 x 1000 fp16: 1.8 times the bytes).
+__device__ __forceinline__ unsigned xcd_run(unsigned id, unsigned n) {
+  const unsigned x = id & 7u, q = n >> 3, r = n & 7u;
+  return x * q + (x < r ? x : r) + (id >> 3);
+}
+
 // Which (b, channels, segment) a thread works on.
 template <class E, int LC, int NG>
 struct Place {
@@ -155,7 +164,7 @@ struct Place {
       seg = 0;
       grp = 0;
     } else {
-      int64_t id = blockIdx.x;
+      int64_t id = xcd_run(blockIdx.x, gridDim.x);
       const int64_t per = a.B * a.nct;
       seg = a.segs > 1 ? (int)(id / per) : 0;
       id -= seg * per;
@@ -658,6 +667,15 @@ __global__ void __launch_bounds__(256) rec_step_kernel(const RecArgs a, float* n
 namespace {
 
 constexpr int REC_LC = 16;  // lanes to a row of a channel tile: 128 bytes
+//   FLAT   T <= 8: a thread per 8 bytes of channels, nothing to join
+//   WAVE   tiles of 64 steps on 128 threads: T <= 64, or workgroups enough without more threads each
+//          (forward + backward us, bf16, D = 2048, WAVE / BLOCK: 64 x 512 steps, 2048 workgroups, 258 /
+//          288; 128 x 256 steps, 4096, 228 / 274; 24 x 2048 steps, 768, 371 / 357; 8 x 4096 steps, 256,
+//          401 / 266)
+//   BLOCK  tiles of 256 steps on 512 threads, one workgroup a compute unit.  Up to 128 workgroups
+//          the time axis is cut so that there are at most 256, one round (65521 x 1000 fp16 forward:
+//          133 us with 16 segments, 151 with 32 in two rounds); above 128 a cut would read the input
+//          twice to fill less than half of the chip more.
 enum { REC_FLAT, REC_WAVE, REC_BLOCK };
 struct RecPlan {
   int kind, steps;  // steps: of a time tile
@@ -670,13 +688,13 @@ RecPlan rec_plan(int dtype, int64_t B, int64_t T, int D) {
   RecPlan p;
   p.nct = (D + REC_LC * V - 1) / (REC_LC * V);
   const int64_t blocks = B * p.nct;
-  p.kind = T <= 8 ? REC_FLAT : T <= 64 || blocks >= 2048 ? REC_WAVE : REC_BLOCK;
+  p.kind = T <= 8 ? REC_FLAT : T <= 64 || blocks >= 1024 ? REC_WAVE : REC_BLOCK;
   p.steps = p.kind == REC_FLAT ? 8 : p.kind == REC_WAVE ? 64 : 256;
   p.tiles = (T + p.steps - 1) / p.steps;
   p.segs = 1;
   p.tps = (int)p.tiles;
-  if (p.kind == REC_BLOCK && blocks < 256 && p.tiles > 1) {
-    const int64_t want = (512 + blocks - 1) / blocks;
+  if (p.kind == REC_BLOCK && blocks <= 128 && p.tiles > 1) {
+    const int64_t want = 256 / blocks;
     p.tps = (int)((p.tiles + want - 1) / want);
     p.segs = (int)((p.tiles + p.tps - 1) / p.tps);
   }
@@ -702,7 +720,7 @@ int rec_fwd_as(hipStream_t s, const RecPlan& p, const RecArgs& a) {
   } else if (p.kind == REC_WAVE) {
     rec_fwd_kernel<E, REC_LC, 8, 8, PART><<<per, 128, 0, s>>>(a);
   } else {
-    if (p.segs > 1) rec_sum_kernel<E, REC_LC, 16, 16, true, PART><<<per * (p.segs - 1), 256, 0, s>>>(a);
+    if (p.segs > 1) rec_sum_kernel<E, REC_LC, 32, 8, true, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
     rec_fwd_kernel<E, REC_LC, 32, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
   }
   return rs_status_after_launch();
@@ -717,7 +735,7 @@ int rec_bwd_as(hipStream_t s, const RecPlan& p, const RecArgs& a) {
   } else if (p.kind == REC_WAVE) {
     rec_bwd_kernel<E, REC_LC, 8, 8, PART><<<per, 128, 0, s>>>(a);
   } else {
-    if (p.segs > 1) rec_sum_kernel<E, REC_LC, 16, 16, false, PART><<<per * (p.segs - 1), 256, 0, s>>>(a);
+    if (p.segs > 1) rec_sum_kernel<E, REC_LC, 32, 8, false, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
     rec_bwd_kernel<E, REC_LC, 32, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
   }
   return rs_status_after_launch();
