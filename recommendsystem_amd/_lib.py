@@ -283,7 +283,7 @@ def call(name: str, *args) -> int:
     if _TRACE and not torch.cuda.is_current_stream_capturing():
         torch.cuda.synchronize()
         print(f"[rs] {name} ok", flush=True)
-    if SIGNATURES[name][0] is _i32 and rc != RS_OK and not name.endswith(("_count", "_blocks")):
+    if rc != RS_OK and SIGNATURES[name][0] is _i32 and not name.endswith(("_count", "_blocks")):
         raise RecsysKernelError(f"{name} returned {rc} ({_ERRS.get(rc, 'hip error')})")
     return rc
 
@@ -306,6 +306,28 @@ def ptr(t) -> int | None:
 def stream_handle() -> int:
     """hipStream_t of torch's current stream on the current device."""
     return torch.cuda.current_stream().cuda_stream
+
+
+def run_on(index: int, fn, *args):
+    """fn(*args, stream) with device `index` current and `stream` its current stream.  Host time
+    counts here (a launch's own is below 5 us): the device is only switched where it has to be, and
+    the stream comes without a Stream object around it."""
+    if index == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def device_index(ref, *others) -> int:
+    """The ROCm device that every tensor (None allowed after the first) is on."""
+    index = ref.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            require_device(ref, t)
+            raise ValueError(f"tensors on different devices: {ref.device} and {t.device}")
+    if index < 0:
+        require_device(ref)
+    return index
 
 
 def require_device(*tensors) -> None:

@@ -321,8 +321,8 @@ def _(ids, offsets, row_base, bucket, hash_mode, combiner, table):
 def layer_norm(x: Tensor, gamma: Tensor, beta: Tensor, epsilon: float) -> tuple[Tensor, Tensor, Tensor]:
     """(y, mean, rstd) of sequence.layer_norm."""
     code = sequence._check_norm(x, gamma, beta, epsilon)
-    with packing.on_device(x, gamma, beta):
-        return sequence._norm_forward(x, gamma, beta, epsilon, code, True, False)[:3]
+    return _lib.run_on(_lib.device_index(x, gamma, beta), sequence._norm_forward, x, gamma, beta,
+                       epsilon, code, True, False)[:3]
 
 
 @layer_norm.register_fake
@@ -335,11 +335,10 @@ def _(x, gamma, beta, epsilon):
 @custom_op("ctr::layer_norm_bwd", mutates_args=())
 def layer_norm_bwd(dy: Tensor, x: Tensor, gamma: Tensor, mean: Tensor,
                    rstd: Tensor) -> tuple[Tensor, Tensor, Tensor]:
-    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
-    with packing.on_device(dy, x, gamma, mean, rstd):
-        dx = sequence._norm_backward(dy, x, None, None, gamma, mean, rstd,
-                                     packing.element_code(x, "layer_norm's input"), dgamma, dbeta, False)
-    return dx, dgamma, dbeta
+    dx, dparams = _lib.run_on(_lib.device_index(dy, x, gamma, mean, rstd), sequence._norm_backward, dy,
+                              x, None, None, gamma, mean, rstd,
+                              packing.element_code(x, "layer_norm's input"), None, False)
+    return dx, dparams[0].clone(), dparams[1].clone()
 
 
 @layer_norm_bwd.register_fake
@@ -370,9 +369,9 @@ def gated_recurrence(v: Tensor, g: Optional[Tensor], h0: Optional[Tensor],
     code = sequence._check_rec(v, g, 3, "gated_recurrence")
     B, T, D = _rec_sizes(v, g)
     sequence._check_state(h0, (B, D), "gated_recurrence: h0")
-    with packing.on_device(v, g, h0, lengths):
-        return sequence._rec_forward(v, g, h0.contiguous() if h0 is not None else None,
-                                     sequence._check_lengths(lengths, B, T), code, True)
+    return _lib.run_on(_lib.device_index(v, g, h0, lengths), sequence._rec_forward, v, g,
+                       h0.contiguous() if h0 is not None else None,
+                       sequence._check_lengths(lengths, B, T), code, True)
 
 
 @gated_recurrence.register_fake
@@ -389,10 +388,10 @@ def gated_recurrence_bwd(dh: Tensor, dlast: Tensor, v: Tensor, g: Optional[Tenso
                          lengths: Optional[Tensor], states: Tensor) -> tuple[Tensor, Tensor, Tensor]:
     """(dv, dg, dh0); with g None dv is the joint rows' gradient and dg is empty."""
     B, T, D = _rec_sizes(v, g)
-    with packing.on_device(v, g, dh, dlast, lengths, states):
-        dv, dg, dh0 = sequence._rec_backward(v, g, sequence._check_lengths(lengths, B, T), states, dh,
-                                             dlast, packing.element_code(v, "gated_recurrence's values"),
-                                             True)
+    dv, dg, dh0 = _lib.run_on(_lib.device_index(v, g, dh, dlast, lengths, states),
+                              sequence._rec_backward, v, g, sequence._check_lengths(lengths, B, T),
+                              states, dh, dlast, packing.element_code(v, "gated_recurrence's values"),
+                              True)
     return dv, v.new_empty(0) if dg is None else dg, dh0
 
 

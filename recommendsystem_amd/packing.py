@@ -12,12 +12,9 @@ nearest whole number: a value is kept to within max|x| / 254 of its block.  Bloc
 """
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
-from . import _lib
-from ._lib import call, ptr, stream_handle
+from ._lib import call, device_index, ptr, run_on
 
 BLOCK = 128
 ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -30,22 +27,10 @@ def element_code(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def on_device(ref: torch.Tensor, *others) -> contextlib.AbstractContextManager:
-    """Checks that every tensor (None allowed) is on ref's ROCm device; a context that makes that
-    device current, whose current stream the kernels then run on."""
-    _lib.require_device(ref)
-    for t in others:
-        if t is not None and t.device != ref.device:
-            _lib.require_device(t)
-            raise ValueError(f"tensors on different devices: {ref.device} and {t.device}")
-    if ref.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(ref.device)
-
-
 def rows_of(t: torch.Tensor) -> torch.Tensor:
     """t [..., D] as a 2-D view with unit column stride, in place where its strides allow it."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -66,12 +51,14 @@ def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     differentiable operation: the codes are kept, not computed with."""
     D = _width(x, "pack8")
     code = element_code(x, "pack8's input")
-    with on_device(x):
-        x2 = rows_of(x.detach())
-        codes = torch.empty(x.shape, device=x.device, dtype=torch.int8)
-        scales = torch.empty(scale_shape(x.shape), device=x.device, dtype=torch.float32)
-        call("rs_pack8", stream_handle(), code, ptr(x2), x2.stride(0), x2.shape[0], D, ptr(codes),
-             ptr(scales))
+    return run_on(device_index(x), _pack, x.detach(), D, code)
+
+
+def _pack(x, D, code, stream):
+    x2 = rows_of(x)
+    codes = x.new_empty(x.shape, dtype=torch.int8)
+    scales = x.new_empty(scale_shape(x.shape), dtype=torch.float32)
+    call("rs_pack8", stream, code, ptr(x2), x2.stride(0), x2.shape[0], D, ptr(codes), ptr(scales))
     return codes, scales
 
 
@@ -85,9 +72,12 @@ def unpack8(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.float32) -> t
                          f"(expected {scale_shape(codes.shape)})")
     if dtype not in ELEMENT_TYPES:
         raise TypeError(f"unpack8: dtype must be float32, bfloat16 or float16, got {dtype}")
-    with on_device(codes, scales):
-        codes, scales = codes.contiguous(), scales.contiguous()
-        y = torch.empty(codes.shape, device=codes.device, dtype=dtype)
-        call("rs_unpack8", stream_handle(), ELEMENT_TYPES[dtype], ptr(codes), ptr(scales),
-             codes.numel() // D, D, ptr(y), D)
+    return run_on(device_index(codes, scales), _unpack, codes, scales, D, dtype)
+
+
+def _unpack(codes, scales, D, dtype, stream):
+    codes, scales = codes.contiguous(), scales.contiguous()
+    y = scales.new_empty(codes.shape, dtype=dtype)
+    call("rs_unpack8", stream, ELEMENT_TYPES[dtype], ptr(codes), ptr(scales), codes.numel() // D, D,
+         ptr(y), D)
     return y

@@ -18,17 +18,38 @@ Rows are float32, bfloat16 or float16; gamma, beta, states and the parameters' g
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, ptr, stream_handle
+from ._lib import call, device_index, ptr, run_on
 from .layers import Dense
-from .packing import element_code, on_device, pack8, rows_of, scale_shape, unpack8  # noqa: F401
+from .packing import element_code, pack8, rows_of, scale_shape, unpack8  # noqa: F401
 from .params import FlatBlock, grads_contiguous
 
 MAX_WIDTH = 32768  # layer_norm's last dimension
+
+
+def _first_order(backward):
+    """backward as it is where no second derivative is asked for, and once_differentiable where one
+    might be (create_graph), whose own work is left out otherwise."""
+    once = once_differentiable(backward)
+    return staticmethod(lambda ctx, *g: once(ctx, *g) if torch.is_grad_enabled() else backward(ctx, *g))
+
+
+# sizes that follow from a shape alone
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace(R, D):
+    return _lib.load().rs_layernorm_bwd_workspace_floats(R, D)
+
+
+@functools.lru_cache(maxsize=1024)
+def _rec_sizes(code, B, T, D):
+    lib = _lib.load()
+    return lib.rs_gated_rec_states_floats(code, B, T, D), lib.rs_gated_rec_workspace_floats(code, B, T, D)
 
 
 # ============================================================================================
@@ -50,35 +71,37 @@ def _check_norm(x, gamma, beta, epsilon):
     return code
 
 
-def _norm_forward(x, gamma, beta, epsilon, code, stats, save_8bit):
+def _norm_forward(x, gamma, beta, epsilon, code, stats, save_8bit, stream):
     x2 = rows_of(x)
     R, D = x2.shape
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = x.new_empty(x.shape)
     mean = rstd = codes = scales = None
     if stats:
-        mean = torch.empty(R, device=x.device, dtype=torch.float32)
-        rstd = torch.empty(R, device=x.device, dtype=torch.float32)
+        mean, rstd = gamma.new_empty(R), gamma.new_empty(R)
     if save_8bit:
-        codes = torch.empty(x.shape, device=x.device, dtype=torch.int8)
-        scales = torch.empty(scale_shape(x.shape), device=x.device, dtype=torch.float32)
-    call("rs_layernorm_fwd", stream_handle(), code, ptr(x2), x2.stride(0), R, D,
-         ptr(gamma.contiguous()), ptr(beta.contiguous()), epsilon, ptr(y), D, ptr(mean), ptr(rstd),
-         ptr(codes), ptr(scales))
+        codes = x.new_empty(x.shape, dtype=torch.int8)
+        scales = gamma.new_empty(scale_shape(x.shape))
+    call("rs_layernorm_fwd", stream, code, x2.data_ptr(), x2.stride(0), R, D,
+         gamma.contiguous().data_ptr(), beta.contiguous().data_ptr(), epsilon, y.data_ptr(), D,
+         ptr(mean), ptr(rstd), ptr(codes), ptr(scales))
     return y, mean, rstd, codes, scales
 
 
-def _norm_backward(dy, x, codes, scales, gamma, mean, rstd, code, dgamma, dbeta, accumulate):
+def _norm_backward(dy, x, codes, scales, gamma, mean, rstd, code, dparams, accumulate, stream):
+    """dx; dparams: [dgamma | dbeta], made here where it is None."""
     dy2 = rows_of(dy)
     R, D = dy2.shape
     x2 = rows_of(x) if x is not None else None
-    dx = torch.empty(dy.shape, device=dy.device, dtype=dy.dtype)
-    ws_n = _lib.load().rs_layernorm_bwd_workspace_floats(R, D)
-    ws = torch.empty(ws_n, device=dy.device, dtype=torch.float32)
-    call("rs_layernorm_bwd", stream_handle(), code, ptr(dy2), dy2.stride(0), ptr(x2),
-         x2.stride(0) if x is not None else 0, ptr(codes), ptr(scales), R, D,
-         ptr(gamma.contiguous()), ptr(mean), ptr(rstd), ptr(dx), D, ptr(dgamma), ptr(dbeta),
-         int(accumulate), ptr(ws), ws_n)
-    return dx
+    dx = dy.new_empty(dy.shape)
+    if dparams is None:
+        dparams = gamma.new_empty(2, D)
+    ws_n = _norm_workspace(R, D)
+    ws = gamma.new_empty(ws_n)
+    call("rs_layernorm_bwd", stream, code, dy2.data_ptr(), dy2.stride(0), ptr(x2),
+         x2.stride(0) if x2 is not None else 0, ptr(codes), ptr(scales), R, D,
+         gamma.contiguous().data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), D,
+         dparams.data_ptr(), dparams.data_ptr() + 4 * D, accumulate, ws.data_ptr(), ws_n)
+    return dx, dparams
 
 
 class _LayerNormFn(torch.autograd.Function):
@@ -86,39 +109,33 @@ class _LayerNormFn(torch.autograd.Function):
     hand autograd None for them (the layers' way); otherwise return them."""
 
     @staticmethod
-    def forward(ctx, x, gamma, beta, epsilon, code, save_8bit, in_place):
-        with on_device(x):
-            y, mean, rstd, codes, scales = _norm_forward(x, gamma, beta, epsilon, code, True, save_8bit)
+    def forward(ctx, x, gamma, beta, epsilon, code, save_8bit, in_place, index):
+        y, mean, rstd, codes, scales = run_on(index, _norm_forward, x, gamma, beta, epsilon, code,
+                                              True, save_8bit)
         ctx.save_for_backward(None if save_8bit else x, codes, scales, gamma, beta, mean, rstd)
-        ctx.code, ctx.in_place = code, in_place
+        ctx.args = code, in_place, index
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, codes, scales, gamma, beta, mean, rstd = ctx.saved_tensors
-        block = grads_contiguous((gamma, beta)) if ctx.in_place else None
-        with on_device(dy):
-            dparams = block if block is not None else torch.empty(
-                2 * gamma.numel(), device=dy.device, dtype=torch.float32)
-            dgamma, dbeta = dparams.view(2, -1)
-            dx = _norm_backward(dy, x, codes, scales, gamma, mean, rstd, ctx.code, dgamma, dbeta,
-                                block is not None)
-        if block is not None:
-            dgamma = dbeta = None
-        return dx, dgamma, dbeta, None, None, None, None
+        code, in_place, index = ctx.args
+        block = grads_contiguous((gamma, beta)) if in_place else None
+        dx, dparams = run_on(index, _norm_backward, dy, x, codes, scales, gamma, mean, rstd, code,
+                             block, block is not None)
+        dgamma, dbeta = dparams.unbind() if block is None else (None, None)
+        return dx, dgamma, dbeta, None, None, None, None, None
 
 
 def _norm(x, gamma, beta, epsilon, save_8bit, in_place):
     code = _check_norm(x, gamma, beta, epsilon)
-    guard = on_device(x, gamma, beta)
+    index = device_index(x, gamma, beta)
     if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
         from . import ops
         if ops.custom_ops_enabled() and not save_8bit:
             return torch.ops.ctr.layer_norm(x, gamma, beta, epsilon)[0]
-        return _LayerNormFn.apply(x, gamma, beta, epsilon, code, save_8bit, in_place)
-    with guard:
-        return _norm_forward(x, gamma, beta, epsilon, code, False, False)[0]
+        return _LayerNormFn.apply(x, gamma, beta, epsilon, code, save_8bit, in_place, index)
+    return run_on(index, _norm_forward, x, gamma, beta, epsilon, code, False, False)[0]
 
 
 def layer_norm(x, gamma, beta, epsilon=1e-5, save_8bit=False):
@@ -198,6 +215,13 @@ def _check_rec(v, g, dims, what):
     return code
 
 
+def _any_grad(*tensors):
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
 def _check_state(state, shape, what):
     if state is None:
         return
@@ -207,74 +231,66 @@ def _check_state(state, shape, what):
         raise ValueError(f"{what} must be {shape}, got {tuple(state.shape)}")
 
 
-def _rec_forward(v, g, h0, lengths, code, keep):
+def _rec_forward(v, g, h0, lengths, code, keep, stream):
     v, g = _halves(v, g)
     v, g = _unit(v), _unit(g)
     B, T, D = v.shape
-    dev, lib = v.device, _lib.load()
-    h = torch.empty(B, T, D, device=dev, dtype=v.dtype)
-    last = torch.empty(B, D, device=dev, dtype=torch.float32)
-    states = None
-    if keep:
-        states = torch.empty(lib.rs_gated_rec_states_floats(code, B, T, D), device=dev,
-                             dtype=torch.float32)
-    ws_n = lib.rs_gated_rec_workspace_floats(code, B, T, D)
-    ws = torch.empty(ws_n, device=dev, dtype=torch.float32) if ws_n else None
-    call("rs_gated_rec_fwd", stream_handle(), code, ptr(v), v.stride(0), v.stride(1), ptr(g),
-         g.stride(0), g.stride(1), B, T, D, ptr(lengths), ptr(h0), ptr(h), ptr(last), ptr(states),
-         ptr(ws), ws_n)
+    n_states, n_ws = _rec_sizes(code, B, T, D)
+    h = v.new_empty((B, T, D))
+    last = v.new_empty((B, D), dtype=torch.float32)
+    states = last.new_empty(n_states) if keep else None
+    ws = last.new_empty(n_ws) if n_ws else None
+    v_sb, v_st, _ = v.stride()
+    g_sb, g_st, _ = g.stride()
+    call("rs_gated_rec_fwd", stream, code, v.data_ptr(), v_sb, v_st, g.data_ptr(), g_sb, g_st, B, T, D,
+         ptr(lengths), ptr(h0), h.data_ptr(), last.data_ptr(), ptr(states), ptr(ws), n_ws)
     return h, last, states
 
 
-def _rec_backward(v, g, lengths, states, dh, dlast, code, want_h0):
+def _rec_backward(v, g, lengths, states, dh, dlast, code, want_h0, stream):
     """(dv, dg, dh0); with g None dv is the gradient of the joint rows and dg None."""
     joint = g is None
     shape = v.shape
     v, g = _halves(v, g)
     v, g = _unit(v), _unit(g)
     B, T, D = v.shape
-    dev, lib = v.device, _lib.load()
-    if joint:
-        dvg = torch.empty(shape, device=dev, dtype=v.dtype)
-        dv, dg = dvg[..., :D], dvg[..., D:]
-    else:
-        dvg = dv = torch.empty(B, T, D, device=dev, dtype=v.dtype)
-        dg = torch.empty(B, T, D, device=dev, dtype=v.dtype)
-    dh0 = torch.empty(B, D, device=dev, dtype=torch.float32) if want_h0 else None
+    dvg = v.new_empty(shape)
+    dv, dg = _halves(dvg, None) if joint else (dvg, v.new_empty(shape))
+    dh0 = states.new_empty((B, D)) if want_h0 else None
+    dh_sb = dh_st = 0
     if dh is not None:
         dh = _unit(dh)
+        dh_sb, dh_st, _ = dh.stride()
     if dlast is not None:
         dlast = dlast.contiguous()
-    ws_n = lib.rs_gated_rec_workspace_floats(code, B, T, D)
-    ws = torch.empty(ws_n, device=dev, dtype=torch.float32) if ws_n else None
-    call("rs_gated_rec_bwd", stream_handle(), code, ptr(v), v.stride(0), v.stride(1), ptr(g),
-         g.stride(0), g.stride(1), B, T, D, ptr(lengths), ptr(states), ptr(dh),
-         dh.stride(0) if dh is not None else 0, dh.stride(1) if dh is not None else 0, ptr(dlast),
-         ptr(dv), dv.stride(0), dv.stride(1), ptr(dg), dg.stride(0), dg.stride(1), ptr(dh0),
-         ptr(ws), ws_n)
+    n_ws = _rec_sizes(code, B, T, D)[1]
+    ws = states.new_empty(n_ws) if n_ws else None
+    v_sb, v_st, _ = v.stride()
+    g_sb, g_st, _ = g.stride()
+    d_sb, d_st, _ = dv.stride()
+    call("rs_gated_rec_bwd", stream, code, v.data_ptr(), v_sb, v_st, g.data_ptr(), g_sb, g_st, B, T, D,
+         ptr(lengths), states.data_ptr(), ptr(dh), dh_sb, dh_st, ptr(dlast), dv.data_ptr(), d_sb, d_st,
+         dg.data_ptr(), d_sb, d_st, ptr(dh0), ptr(ws), n_ws)
     return dvg, None if joint else dg, dh0
 
 
 class _RecurrenceFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, v, g, h0, lengths, code):
+    def forward(ctx, v, g, h0, lengths, code, index):
         ctx.set_materialize_grads(False)
-        with on_device(v):
-            h, last, states = _rec_forward(v, g, h0, lengths, code, True)
+        h, last, states = run_on(index, _rec_forward, v, g, h0, lengths, code, True)
         ctx.save_for_backward(v, g, lengths, states)
-        ctx.code = code
+        ctx.args = code, index
         return h, last
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dh, dlast):
         v, g, lengths, states = ctx.saved_tensors
         if dh is None and dlast is None:
-            return None, None, None, None, None
-        with on_device(v):
-            dv, dg, dh0 = _rec_backward(v, g, lengths, states, dh, dlast, ctx.code,
-                                        ctx.needs_input_grad[2])
-        return dv, dg, dh0, None, None
+            return None, None, None, None, None, None
+        code, index = ctx.args
+        return (*run_on(index, _rec_backward, v, g, lengths, states, dh, dlast, code,
+                        ctx.needs_input_grad[2]), None, None, None)
 
 
 def _check_lengths(lengths, B, T):
@@ -302,17 +318,16 @@ def gated_recurrence(v, g=None, h0=None, lengths=None):
     code = _check_rec(v, g, 3, "gated_recurrence")
     B, T, D = v.shape if g is not None else (*v.shape[:2], v.shape[2] // 2)
     _check_state(h0, (B, D), "gated_recurrence: h0")
-    guard = on_device(v, g, h0, lengths)
+    index = device_index(v, g, h0, lengths)
     lengths = _check_lengths(lengths, B, T)
     if h0 is not None:
         h0 = h0.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (v, g, h0)):
+    if torch.is_grad_enabled() and _any_grad(v, g, h0):
         from . import ops
         if ops.custom_ops_enabled():
             return tuple(torch.ops.ctr.gated_recurrence(v, g, h0, lengths)[:2])
-        return _RecurrenceFn.apply(v, g, h0, lengths, code)
-    with guard:
-        return _rec_forward(v, g, h0, lengths, code, False)[:2]
+        return _RecurrenceFn.apply(v, g, h0, lengths, code, index)
+    return run_on(index, _rec_forward, v, g, h0, lengths, code, False)[:2]
 
 
 def gated_recurrence_step(v, g=None, state=None, out=None):
@@ -326,19 +341,22 @@ def gated_recurrence_step(v, g=None, state=None, out=None):
     _check_state(out, (B, D), "gated_recurrence_step: out")
     if out is not None and not out.is_contiguous():
         raise ValueError("gated_recurrence_step: out must be contiguous")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (v, g, state, out)):
+    if torch.is_grad_enabled() and _any_grad(v, g, state, out):
         raise RuntimeError("gated_recurrence_step has no backward: call it under torch.no_grad(), or "
                            "gated_recurrence with one step")
-    with on_device(v, g, state, out):
-        v, g = _halves(v, g)
-        v, g = _unit(v), _unit(g)
-        if state is not None and not state.is_contiguous():
-            state = state.contiguous()
-        h = torch.empty(B, D, device=v.device, dtype=v.dtype)
-        if out is None:
-            out = torch.empty(B, D, device=v.device, dtype=torch.float32)
-        call("rs_gated_rec_step", stream_handle(), code, ptr(v), v.stride(0), ptr(g), g.stride(0),
-             B, D, ptr(state), ptr(h), ptr(out))
+    return run_on(device_index(v, g, state, out), _rec_step, v, g, state, out, B, D, code)
+
+
+def _rec_step(v, g, state, out, B, D, code, stream):
+    v, g = _halves(v, g)
+    v, g = _unit(v), _unit(g)
+    if state is not None:
+        state = state.contiguous()
+    h = v.new_empty((B, D))
+    if out is None:
+        out = v.new_empty((B, D), dtype=torch.float32)
+    call("rs_gated_rec_step", stream, code, v.data_ptr(), v.stride(0), g.data_ptr(), g.stride(0), B, D,
+         ptr(state), h.data_ptr(), out.data_ptr())
     return h, out
 
 
