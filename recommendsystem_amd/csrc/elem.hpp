@@ -258,12 +258,12 @@ __device__ __forceinline__ uint32_t group_umax(uint32_t v) {
   return v;
 }
 
-// The largest magnitude of V elements as a bit pattern: the order of the patterns is that of the
-// numbers, with NaN above infinity
+// The largest magnitude of V elements (NaN if one is NaN) as a bit pattern: the order of the patterns
+// is that of the numbers, with NaN above infinity
 template <int V>
 __device__ __forceinline__ uint32_t top_bits(const float* x) {
-  uint32_t t = 0;
+  float t = fabsf(x[0]);
 #pragma unroll
-  for (int j = 0; j < V; ++j) t = max(t, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-  return t;
+  for (int j = 1; j < V; ++j) t = __builtin_elementwise_maximum(t, fabsf(x[j]));
+  return __float_as_uint(t) & 0x7FFFFFFFu;
 }

@@ -2,19 +2,18 @@
 //   mean = sum x / D, rstd = 1 / sqrt(sum (x - mean)^2 / D + eps), xh = (x - mean) rstd
 //   y = xh gamma + beta
 //   w = dy gamma;  dx = rstd (w - mean(w) - xh mean(w xh));  dgamma = sum_rows dy xh;  dbeta = sum_rows dy
-// All sums are held in fp32.  The mean is corrected by the mean of x - mean (which subtracts
-// without error when the row's spread is small against its offset), in both passes, so a row with
-// a large offset loses nothing to the rounding of its own mean.
+// All sums are held in fp32.  The forward sums x - x[0] and the mean is corrected by the mean of x -
+// mean, in both passes (both subtract without error when the row's spread is small against its
+// offset), so a row with a large offset loses nothing to the rounding of its own mean, and a
+// constant row is normalised to exact zeros.
 //
-// Bound by memory.  A row lives in the registers of TPR threads (4 .. 64 lanes of a wave, or a
-// workgroup of 256 or 512), NCH x 16 bytes each, so it is read once; workgroups stay and walk the
-// rows, with gamma and beta in registers and the next row's loads in flight.  In the backward every
+// Bound by memory.  A row lives in the registers of TPR threads (1 .. 64 lanes of a wave, or 2 to 8
+// waves), NCH x 16 bytes each, so it is read once; workgroups stay and walk the rows, with gamma and beta in registers and the next row's loads in flight.  In the backward every
 // thread also keeps its columns' share of dgamma and dbeta in registers over all of its rows; one
 // partial row a workgroup then goes to the workspace and a second launch adds them in a fixed order.
 #include "elem.hpp"
 
 #define LN_MAX_D 32768
-#define LN_REG_D 16384  // rows up to here fit the registers of one workgroup
 
 namespace {
 
@@ -32,44 +31,48 @@ struct LnArgs {
   float *dgamma, *dbeta, *ws;
 };
 
-// sums of v[0..N) over the TPR threads of a row, in each of them.  red: [2][N][waves], used in turn
-// (flip), so one barrier a call is enough.
-template <int N, int TPR>
-__device__ __forceinline__ void row_sum(float* v, float* red, int& flip) {
-#pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = group_sum<(TPR < 64 ? TPR : 64)>(v[k]);
-  if (TPR > 64) {
-    constexpr int W = TPR / 64;
-    float* r = red + flip * N * W;
-    flip ^= 1;
-    if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-      for (int k = 0; k < N; ++k) r[k * W + (threadIdx.x >> 6)] = v[k];
-    }
-    lds_barrier();
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      v[k] = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) v[k] += r[k * W + w];
-    }
-  }
-}
-
 template <int TPR>
 struct LnShape {
   static constexpr int THREADS = TPR < 256 ? 256 : TPR;
   static constexpr int RPB = THREADS / TPR;  // rows a workgroup holds at a time
 };
 
+// sums of v[0..N) over the TPR threads of a row, in each of them.  red: two buffers of N floats a
+// wave, used in turn (flip), so one barrier a call is enough.
+template <int N, int TPR>
+__device__ __forceinline__ void row_sum(float* v, float* red, int& flip) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = group_sum<(TPR < 64 ? TPR : 64)>(v[k]);
+  if (TPR > 64) {
+    constexpr int W = TPR / 64, ALL = LnShape<TPR>::THREADS / 64;
+    float* r = red + flip * N * ALL;
+    const int wave = wave_id();
+    flip ^= 1;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) r[k * ALL + wave] = v[k];
+    }
+    lds_barrier();
+    r += wave / W * W;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) v[k] += r[k * ALL + w];
+    }
+  }
+}
+
 }  // namespace
 
 template <class E, int TPR, int NCH, bool PACK>
 __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_fwd_kernel(const LnArgs a) {
   constexpr int V = E::V, RPB = LnShape<TPR>::RPB;
-  constexpr int LB = RS_PACK_BLOCK / V < TPR ? RS_PACK_BLOCK / V : TPR;  // lanes of an 8-bit block
+  // an 8-bit block is 16 bytes of LB lanes, CPB times over
+  constexpr int LB = RS_PACK_BLOCK / V < TPR ? RS_PACK_BLOCK / V : TPR;
+  constexpr int CPB = RS_PACK_BLOCK / V / LB;
   typedef typename E::T X;
-  __shared__ float red[2 * 2 * (TPR + 63) / 64];
+  __shared__ float red[2 * 2 * LnShape<TPR>::THREADS / 64];
   const int tr = (int)threadIdx.x % TPR, nb = (a.D + RS_PACK_BLOCK - 1) / RS_PACK_BLOCK;
   const float inv = 1.0f / (float)a.D;
   int flip = 0;
@@ -83,6 +86,7 @@ __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_fwd_kernel(const LnA
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t row = (int64_t)blockIdx.x * RPB + (int)threadIdx.x / TPR;
   Raw next[NCH];
+  float next0;
   auto load = [&](int64_t r) {  // (behind the last row: the last row again, and not stored)
     const X* p = (const X*)a.x + (r < a.rows ? r : a.rows - 1) * a.ldx;
 #pragma unroll
@@ -90,6 +94,7 @@ __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_fwd_kernel(const LnA
       const int col = (c * TPR + tr) * V;
       load16<E, true>(next[c], p + col, a.D - col, true, 0u);
     }
+    next0 = E::load(p[0]);
   };
   load(row);
   // every thread of the workgroup runs the same number of rounds
@@ -97,28 +102,40 @@ __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_fwd_kernel(const LnA
     float x[NCH][V];
 #pragma unroll
     for (int c = 0; c < NCH; ++c) E::unpack(next[c].w, x[c]);
+    const float x0 = next0;
     if (first + step < a.rows) load(row + step);
-    float s[1] = {0.f}, q[2] = {0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < NCH; ++c)
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += x[c][j];
-    row_sum<1, TPR>(s, red, flip);
-    const float m0 = s[0] * inv;
     const bool live = row < a.rows;
     if (PACK) {
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        const int col = (c * TPR + tr) * V, nv = a.D - col;
-        const float sc = pack8_scale(group_umax<LB>(top_bits<V>(x[c])));
-        uint32_t w[V / 4];
-        pack8_codes<V>(x[c], sc, pack8_inverse(sc), w);
-        if (live) {
-          store_codes<V>(a.codes + row * a.D + col, w, nv);
-          if (tr % LB == 0 && nv > 0) a.scales[row * nb + col / RS_PACK_BLOCK] = sc;
+      for (int c0 = 0; c0 < NCH; c0 += CPB) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = c0; c < c0 + CPB && c < NCH; ++c) top = max(top, top_bits<V>(x[c]));
+        const float sc = pack8_scale(group_umax<LB>(top)), inv8 = pack8_inverse(sc);
+#pragma unroll
+        for (int c = c0; c < c0 + CPB && c < NCH; ++c) {
+          const int col = (c * TPR + tr) * V, nv = a.D - col;
+          uint32_t w[V / 4];
+          pack8_codes<V>(x[c], sc, inv8, w);
+          if (live) {
+            store_codes<V>(a.codes + row * a.D + col, w, nv);
+            if (c == c0 && tr % LB == 0 && nv > 0) a.scales[row * nb + col / RS_PACK_BLOCK] = sc;
+          }
         }
       }
     }
+    float s[1] = {0.f}, q[2] = {0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int nv = a.D - (c * TPR + tr) * V;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        x[c][j] -= x0;
+        s[0] += j < nv ? x[c][j] : 0.f;
+      }
+    }
+    row_sum<1, TPR>(s, red, flip);
+    const float m0 = s[0] * inv;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int nv = a.D - (c * TPR + tr) * V;
@@ -143,7 +160,7 @@ __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_fwd_kernel(const LnA
         if (col < a.D) store16<E>((X*)a.y + row * a.ldy + col, y, a.D - col);
       }
       if (tr == 0 && a.mean) {
-        a.mean[row] = m0 + dl;
+        a.mean[row] = x0 + (m0 + dl);
         a.rstd[row] = rs;
       }
     }
@@ -155,7 +172,7 @@ template <class E, int TPR, int NCH, bool Q8>
 __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_bwd_kernel(const LnArgs a) {
   constexpr int V = E::V, RPB = LnShape<TPR>::RPB, THREADS = LnShape<TPR>::THREADS;
   typedef typename E::T X;
-  __shared__ float red[2 * 3 * (TPR + 63) / 64];
+  __shared__ float red[2 * 3 * LnShape<TPR>::THREADS / 64];
   __shared__ float fold[RPB > 1 ? THREADS * V : 1];
   const int tr = (int)threadIdx.x % TPR, nb = (a.D + RS_PACK_BLOCK - 1) / RS_PACK_BLOCK;
   const float inv = 1.0f / (float)a.D;
@@ -242,7 +259,13 @@ __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_bwd_kernel(const LnA
     for (int c = 0; c < NCH; ++c) {
       const int col = (c * TPR + tr) * V;
       float* v = k ? ab[c] : ag[c];
+      // over the rows of a wave by exchanges, over the waves through LDS
+#pragma unroll
+      for (int o = TPR; o < 64; o <<= 1)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += __shfl_xor(v[j], o, 64);
       if (RPB > 1) {
+        constexpr int SPAN = TPR < 64 ? 64 : TPR, N = THREADS / SPAN;  // threads between equal columns
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < V; ++j) fold[j * THREADS + threadIdx.x] = v[j];
@@ -251,7 +274,8 @@ __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_bwd_kernel(const LnA
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             v[j] = 0.f;
-            for (int r = 0; r < RPB; ++r) v[j] += fold[j * THREADS + r * TPR + tr];
+#pragma unroll
+            for (int r = 0; r < N; ++r) v[j] += fold[j * THREADS + r * SPAN + tr];
           }
         }
       }
@@ -284,36 +308,81 @@ __global__ void __launch_bounds__(1024) ln_params_kernel(const float* __restrict
 }
 
 // ---------------------------------------------------------------------------------------------
-// Rows beyond LN_REG_D: one workgroup a row, which it reads three times (from cache after the first)
+// Wider rows: one workgroup a row, which it reads two or three times (from cache after the first);
+// the parameters' gradients are summed by columns in a launch of their own.
 // ---------------------------------------------------------------------------------------------
+namespace {
+constexpr int LN_WIDE = 1024;  // threads
+
+// f(x, col, nv) for 16 bytes after 16 bytes of a row
+template <class E, class F>
+__device__ __forceinline__ void for_row(const typename E::T* p, int D, F f) {
+#pragma unroll 2
+  for (int col = (int)threadIdx.x * E::V; col < D; col += LN_WIDE * E::V) {
+    Raw r;
+    float x[E::V];
+    load16<E, true>(r, p + col, D - col, true, 0u);
+    E::unpack(r.w, x);
+    f(x, col, D - col);
+  }
+}
+// the row's input at col: 16 bytes of x, or as many codes
+template <class E, bool Q8>
+__device__ __forceinline__ void ln_in(const LnArgs& a, int nb, int64_t r, int col, float* x) {
+  if (Q8) {
+    uint32_t w[E::V / 4];
+    load_codes<E::V>(w, a.codes + r * a.D + col, a.D - col);
+    unpack_codes<E::V>(w, a.scales[r * nb + col / RS_PACK_BLOCK], x);
+  } else {
+    Raw q;
+    load16<E, true>(q, (const typename E::T*)a.x + r * a.ldx + col, a.D - col, true, 0u);
+    E::unpack(q.w, x);
+  }
+}
+}  // namespace
+
 template <class E>
-__global__ void __launch_bounds__(256) ln_wide_fwd_kernel(const LnArgs a) {
+__global__ void __launch_bounds__(LN_WIDE) ln_wide_fwd_kernel(const LnArgs a) {
   typedef typename E::T X;
-  __shared__ float red[2 * 2 * 4];
+  constexpr int V = E::V;
+  __shared__ float red[2 * 2 * LN_WIDE / 64];
   int flip = 0;
   const int D = a.D, nb = (D + RS_PACK_BLOCK - 1) / RS_PACK_BLOCK;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const X* xr = (const X*)a.x + r * a.ldx;
     float s[1] = {0.f}, q[2] = {0.f, 0.f};
-    for (int c = threadIdx.x; c < D; c += 256) s[0] += E::load(xr[c]);
-    row_sum<1, 256>(s, red, flip);
+    const float x0 = E::load(xr[0]);
+    for_row<E>(xr, D, [&](const float* x, int, int nv) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[0] += j < nv ? x[j] - x0 : 0.f;
+    });
+    row_sum<1, LN_WIDE>(s, red, flip);
     const float m0 = s[0] / (float)D;
-    for (int c = threadIdx.x; c < D; c += 256) {
-      const float d = E::load(xr[c]) - m0;
-      q[0] += d;
-      q[1] = fmaf(d, d, q[1]);
-    }
-    row_sum<2, 256>(q, red, flip);
+    for_row<E>(xr, D, [&](const float* x, int, int nv) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = j < nv ? x[j] - x0 - m0 : 0.f;
+        q[0] += d;
+        q[1] = fmaf(d, d, q[1]);
+      }
+    });
+    row_sum<2, LN_WIDE>(q, red, flip);
     const float dl = q[0] / (float)D, var = q[1] / (float)D - dl * dl;
     const float rs = 1.0f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
-    for (int c = threadIdx.x; c < D; c += 256)
-      ((X*)a.y)[r * a.ldy + c] = E::store(fmaf((E::load(xr[c]) - m0 - dl) * rs, a.gamma[c], a.beta[c]));
+    for_row<E>(xr, D, [&](const float* x, int col, int nv) {
+      float y[V], gm[V], bt[V];
+      load_f<V>(gm, a.gamma + col, nv);
+      load_f<V>(bt, a.beta + col, nv);
+#pragma unroll
+      for (int j = 0; j < V; ++j) y[j] = fmaf((x[j] - x0 - m0 - dl) * rs, gm[j], bt[j]);
+      store16<E>((X*)a.y + r * a.ldy + col, y, nv);
+    });
     if (threadIdx.x == 0 && a.mean) {
-      a.mean[r] = m0 + dl;
+      a.mean[r] = x0 + (m0 + dl);
       a.rstd[r] = rs;
     }
     if (a.codes) {  // 32 lanes x 4 elements a block
-      for (int b = (int)threadIdx.x >> 5; b < nb; b += 8) {
+      for (int b = (int)threadIdx.x >> 5; b < nb; b += LN_WIDE / 32) {
         const int c = b * RS_PACK_BLOCK + ((int)threadIdx.x & 31) * 4;
         float x[4];
 #pragma unroll
@@ -328,66 +397,72 @@ __global__ void __launch_bounds__(256) ln_wide_fwd_kernel(const LnArgs a) {
   }
 }
 
-template <class E, bool Q8>
-__device__ __forceinline__ float ln_in(const LnArgs& a, int nb, int64_t r, int c) {
-  return Q8 ? (float)a.codes[r * a.D + c] * a.scales[r * nb + c / RS_PACK_BLOCK]
-            : E::load(((const typename E::T*)a.x)[r * a.ldx + c]);
-}
-
 // dx of a row, and its corrected mean into ws
 template <class E, bool Q8>
-__global__ void __launch_bounds__(256) ln_wide_bwd_kernel(const LnArgs a) {
+__global__ void __launch_bounds__(LN_WIDE) ln_wide_bwd_kernel(const LnArgs a) {
   typedef typename E::T X;
-  __shared__ float red[2 * 3 * 4];
+  constexpr int V = E::V;
+  __shared__ float red[2 * 3 * LN_WIDE / 64];
   int flip = 0;
   const int D = a.D, nb = (D + RS_PACK_BLOCK - 1) / RS_PACK_BLOCK;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const X* dy = (const X*)a.dy + r * a.lddy;
     const float m = a.mean[r], rs = a.rstd[r];
     float s[3] = {0.f, 0.f, 0.f};
-    for (int c = threadIdx.x; c < D; c += 256) {
-      const float w = E::load(dy[c]) * a.gamma[c], d = ln_in<E, Q8>(a, nb, r, c) - m;
-      s[0] += w;
-      s[1] = fmaf(w, d, s[1]);
-      s[2] += d;
-    }
-    row_sum<3, 256>(s, red, flip);
+    for_row<E>(dy, D, [&](const float* y, int col, int nv) {
+      float gm[V], x[V];
+      load_f<V>(gm, a.gamma + col, nv);
+      ln_in<E, Q8>(a, nb, r, col, x);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float w = y[j] * gm[j], d = j < nv ? x[j] - m : 0.f;
+        s[0] += w;
+        s[1] = fmaf(w, d, s[1]);
+        s[2] += d;
+      }
+    });
+    row_sum<3, LN_WIDE>(s, red, flip);
     const float dl = Q8 ? 0.f : s[2] / (float)D;
     const float c1 = s[0] / (float)D, c2 = (s[1] / (float)D - dl * c1) * rs * rs;
-    for (int c = threadIdx.x; c < D; c += 256) {
-      const float d = ln_in<E, Q8>(a, nb, r, c) - m - dl;
-      ((X*)a.dx)[r * a.lddx + c] = E::store(rs * (fmaf(E::load(dy[c]), a.gamma[c], -c1) - d * c2));
-    }
+    for_row<E>(dy, D, [&](const float* y, int col, int nv) {
+      float gm[V], x[V], o[V];
+      load_f<V>(gm, a.gamma + col, nv);
+      ln_in<E, Q8>(a, nb, r, col, x);
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = rs * (fmaf(y[j], gm[j], -c1) - (x[j] - m - dl) * c2);
+      store16<E>((X*)a.dx + r * a.lddx + col, o, nv);
+    });
     if (threadIdx.x == 0) a.ws[r] = m + dl;
   }
 }
 
-// dgamma and dbeta of 4 columns
+// Partial rows [dgamma | dbeta] of 16 bytes of columns a thread, over every gridDim.y-th row
 template <class E, bool Q8>
-__global__ void __launch_bounds__(256) ln_wide_params_kernel(const LnArgs a) {
+__global__ void __launch_bounds__(64) ln_wide_params_kernel(const LnArgs a) {
+  constexpr int V = E::V;
   const int nb = (a.D + RS_PACK_BLOCK - 1) / RS_PACK_BLOCK;
-  const int c = (int)blockIdx.x * 4 + (int)(threadIdx.x & 3);
-  float s[2] = {0.f, 0.f};
-  if (c < a.D)
-    for (int64_t r = threadIdx.x >> 2; r < a.rows; r += 64) {
-      const float g = E::load(((const typename E::T*)a.dy)[r * a.lddy + c]);
-      s[0] = fmaf(g, (ln_in<E, Q8>(a, nb, r, c) - a.ws[r]) * a.rstd[r], s[0]);
-      s[1] += g;
-    }
-  __shared__ float red[2][256];
-  red[0][threadIdx.x] = s[0];
-  red[1][threadIdx.x] = s[1];
-  for (int o = 128; o >= 4; o >>= 1) {
-    __syncthreads();
-    if ((int)threadIdx.x < o) {
-      red[0][threadIdx.x] += red[0][threadIdx.x + o];
-      red[1][threadIdx.x] += red[1][threadIdx.x + o];
+  const int col = ((int)blockIdx.x * 64 + (int)threadIdx.x) * V, nv = a.D - col;
+  if (nv <= 0) return;
+  float ag[V], ab[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) ag[j] = ab[j] = 0.f;
+#pragma unroll 4
+  for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
+    Raw q;
+    float y[V], x[V];
+    load16<E, true>(q, (const typename E::T*)a.dy + r * a.lddy + col, nv, true, 0u);
+    E::unpack(q.w, y);
+    ln_in<E, Q8>(a, nb, r, col, x);
+    const float m = a.ws[r], rs = a.rstd[r];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      ag[j] = fmaf(y[j], (x[j] - m) * rs, ag[j]);
+      ab[j] += y[j];
     }
   }
-  if (threadIdx.x < 4 && c < a.D) {
-    a.dgamma[c] = red[0][threadIdx.x] + (a.accumulate ? a.dgamma[c] : 0.f);
-    a.dbeta[c] = red[1][threadIdx.x] + (a.accumulate ? a.dbeta[c] : 0.f);
-  }
+  float* part = a.ws + a.rows + (int64_t)blockIdx.y * 2 * a.D + col;
+  store_f<V>(part, ag, nv);
+  store_f<V>(part + a.D, ab, nv);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -395,10 +470,21 @@ __global__ void __launch_bounds__(256) ln_wide_params_kernel(const LnArgs a) {
 // ---------------------------------------------------------------------------------------------
 namespace {
 
-// threads of a row
-int ln_tpr(int D, int V) {
-  const int ch = (D + V - 1) / V;  // 16-byte pieces; at most 4 a thread (fp32 rows over 8192: 8)
-  return ch <= 4 ? 4 : ch <= 8 ? 8 : ch <= 16 ? 16 : ch <= 32 ? 32 : ch <= 256 ? 64 : ch <= 1024 ? 256 : 512;
+// (threads of a row, 16-byte pieces a thread), the first that holds the row: at most a third of the
+// lanes without work.  Few threads with several pieces rather than many with one: fewer exchanges.
+#define LN_SHAPES(X)                                                                            \
+  X(1, 1) X(1, 2) X(1, 3) X(2, 2) X(2, 3) X(4, 2) X(4, 3) X(8, 2) X(8, 3) X(16, 2) X(16, 3)     \
+  X(32, 2) X(32, 3) X(64, 2) X(64, 3) X(64, 4) X(128, 3) X(128, 4) X(256, 3) X(256, 4)          \
+  X(512, 3) X(512, 4)
+
+int ln_pieces(int D, int V) { return (D + V - 1) / V; }
+
+int ln_tpr(int pieces) {
+#define LN_TPR(TPR, NCH) \
+  if (pieces <= TPR * NCH) return TPR;
+  LN_SHAPES(LN_TPR)
+#undef LN_TPR
+  return 0;  // wider
 }
 
 int64_t ln_grid(int64_t rows, int tpr, int64_t most) {
@@ -406,58 +492,66 @@ int64_t ln_grid(int64_t rows, int tpr, int64_t most) {
   return n < most ? n : most;
 }
 
-// workgroups of the backward: two a compute unit, which is what its registers allow
-int64_t ln_bwd_grid(int64_t rows, int D, int V) { return ln_grid(rows, ln_tpr(D, V), 512); }
-
-// KERNEL<E, TPR, NCH, FLAG> for the width
-#define LN_LAUNCH(KERNEL, FLAG)                                                                \
-  do {                                                                                         \
-    const int ch = (a.D + E::V - 1) / E::V, tpr = ln_tpr(a.D, E::V);                           \
-    if (tpr == 4) KERNEL<E, 4, 1, FLAG><<<grid, 256, 0, s>>>(a);                               \
-    else if (tpr == 8) KERNEL<E, 8, 1, FLAG><<<grid, 256, 0, s>>>(a);                          \
-    else if (tpr == 16) KERNEL<E, 16, 1, FLAG><<<grid, 256, 0, s>>>(a);                        \
-    else if (tpr == 32) KERNEL<E, 32, 1, FLAG><<<grid, 256, 0, s>>>(a);                        \
-    else if (tpr == 64 && ch <= 64) KERNEL<E, 64, 1, FLAG><<<grid, 256, 0, s>>>(a);            \
-    else if (tpr == 64 && ch <= 128) KERNEL<E, 64, 2, FLAG><<<grid, 256, 0, s>>>(a);           \
-    else if (tpr == 64) KERNEL<E, 64, 4, FLAG><<<grid, 256, 0, s>>>(a);                        \
-    else if (tpr == 256 && ch <= 512) KERNEL<E, 256, 2, FLAG><<<grid, 256, 0, s>>>(a);         \
-    else if (tpr == 256) KERNEL<E, 256, 4, FLAG><<<grid, 256, 0, s>>>(a);                      \
-    else if (ch <= 2048) KERNEL<E, 512, 4, FLAG><<<grid, 512, 0, s>>>(a);                      \
-    else KERNEL<E, 512, E::V == 4 ? 8 : 4, FLAG><<<grid, 512, 0, s>>>(a);                      \
-  } while (0)
+// partial rows of the parameters' gradients: two workgroups a compute unit, which is what the
+// backward's registers allow; for wider rows as many groups of rows as give 1024 or so waves
+int64_t ln_parts(int64_t rows, int D, int V) {
+  const int tpr = ln_tpr(ln_pieces(D, V));
+  if (tpr) return ln_grid(rows, tpr, 512);
+  const int64_t most = 65536 / ln_pieces(D, V) + 1;
+  return rows < most ? rows : most;
+}
 
 template <class E>
 int ln_fwd(hipStream_t s, const LnArgs& a) {
-  if (a.D > LN_REG_D) {
-    ln_wide_fwd_kernel<E><<<(unsigned)(a.rows < 65536 ? a.rows : 65536), 256, 0, s>>>(a);
+  const int pieces = ln_pieces(a.D, E::V), tpr = ln_tpr(pieces);
+  if (!tpr) {
+    ln_wide_fwd_kernel<E><<<(unsigned)(a.rows < 65536 ? a.rows : 65536), LN_WIDE, 0, s>>>(a);
     return rs_status_after_launch();
   }
-  const unsigned grid = (unsigned)ln_grid(a.rows, ln_tpr(a.D, E::V), 2048);
-  if (a.codes) LN_LAUNCH(ln_fwd_kernel, true);
-  else LN_LAUNCH(ln_fwd_kernel, false);
-  return rs_status_after_launch();
+  const unsigned grid = (unsigned)ln_grid(a.rows, tpr, 2048);
+#define LN_FWD(TPR, NCH)                                                               \
+  if (pieces <= TPR * NCH) {                                                           \
+    if (a.codes) ln_fwd_kernel<E, TPR, NCH, true><<<grid, LnShape<TPR>::THREADS, 0, s>>>(a); \
+    else ln_fwd_kernel<E, TPR, NCH, false><<<grid, LnShape<TPR>::THREADS, 0, s>>>(a);  \
+    return rs_status_after_launch();                                                   \
+  }
+  LN_SHAPES(LN_FWD)
+#undef LN_FWD
+  return RS_ERR_UNSUPPORTED;
+}
+
+template <class E>
+void ln_bwd_rows(hipStream_t s, const LnArgs& a, unsigned grid) {
+  const int pieces = ln_pieces(a.D, E::V);
+#define LN_BWD(TPR, NCH)                                                               \
+  if (pieces <= TPR * NCH) {                                                           \
+    if (a.codes) ln_bwd_kernel<E, TPR, NCH, true><<<grid, LnShape<TPR>::THREADS, 0, s>>>(a); \
+    else ln_bwd_kernel<E, TPR, NCH, false><<<grid, LnShape<TPR>::THREADS, 0, s>>>(a);  \
+    return;                                                                            \
+  }
+  LN_SHAPES(LN_BWD)
+#undef LN_BWD
 }
 
 template <class E>
 int ln_bwd(hipStream_t s, const LnArgs& a) {
-  if (a.D > LN_REG_D) {
-    const unsigned grid = (unsigned)(a.rows < 65536 ? a.rows : 65536), cols = (unsigned)((a.D + 3) / 4);
+  const bool wide = !ln_tpr(ln_pieces(a.D, E::V));
+  const unsigned parts = (unsigned)ln_parts(a.rows, a.D, E::V);
+  if (a.rows && wide) {
+    const unsigned grid = (unsigned)(a.rows < 65536 ? a.rows : 65536);
+    const dim3 cols((unsigned)((ln_pieces(a.D, E::V) + 63) / 64), parts);
     if (a.codes) {
-      if (a.rows) ln_wide_bwd_kernel<E, true><<<grid, 256, 0, s>>>(a);
-      ln_wide_params_kernel<E, true><<<cols, 256, 0, s>>>(a);
+      ln_wide_bwd_kernel<E, true><<<grid, LN_WIDE, 0, s>>>(a);
+      ln_wide_params_kernel<E, true><<<cols, 64, 0, s>>>(a);
     } else {
-      if (a.rows) ln_wide_bwd_kernel<E, false><<<grid, 256, 0, s>>>(a);
-      ln_wide_params_kernel<E, false><<<cols, 256, 0, s>>>(a);
+      ln_wide_bwd_kernel<E, false><<<grid, LN_WIDE, 0, s>>>(a);
+      ln_wide_params_kernel<E, false><<<cols, 64, 0, s>>>(a);
     }
-    return rs_status_after_launch();
+  } else if (a.rows) {
+    ln_bwd_rows<E>(s, a, parts);
   }
-  const unsigned grid = (unsigned)ln_bwd_grid(a.rows, a.D, E::V);
-  if (grid) {
-    if (a.codes) LN_LAUNCH(ln_bwd_kernel, true);
-    else LN_LAUNCH(ln_bwd_kernel, false);
-  }
-  ln_params_kernel<<<(unsigned)((2 * a.D + 31) / 32), 1024, 0, s>>>(a.ws, (int)grid, a.D, a.dgamma,
-                                                                    a.dbeta, a.accumulate);
+  ln_params_kernel<<<(unsigned)((2 * a.D + 31) / 32), 1024, 0, s>>>(
+      wide ? a.ws + a.rows : a.ws, (int)parts, a.D, a.dgamma, a.dbeta, a.accumulate);
   return rs_status_after_launch();
 }
 
@@ -477,12 +571,15 @@ RS_API int rs_layernorm_fwd(void* stream, int dtype, const void* x, int64_t ld_x
   return RS_DISPATCH_ELEM(dtype, ln_fwd, rs_stream(stream), a);
 }
 
-// the partial rows of whichever type needs more
+// for whichever element size needs more
 RS_API int64_t rs_layernorm_bwd_workspace_floats(int64_t rows, int D) {
   if (rows < 0 || D <= 0 || D > LN_MAX_D) return 0;
-  if (D > LN_REG_D) return rows;
-  const int64_t g4 = ln_bwd_grid(rows, D, 4), g8 = ln_bwd_grid(rows, D, 8);
-  return (g4 > g8 ? g4 : g8) * 2 * D;
+  int64_t most = 0;
+  for (int V = 4; V <= 8; V += 4) {
+    const int64_t n = ln_parts(rows, D, V) * 2 * D + (ln_tpr(ln_pieces(D, V)) ? 0 : rows);
+    if (n > most) most = n;
+  }
+  return most;
 }
 
 RS_API int rs_layernorm_bwd(void* stream, int dtype, const void* dy, int64_t ld_dy, const void* x,

@@ -91,7 +91,9 @@ int pack8(hipStream_t s, const void* x, int64_t ld, int64_t rows, int D, int8_t*
   const int nb = (D + RS_PACK_BLOCK - 1) / RS_PACK_BLOCK, ch = (D + E::V - 1) / E::V;
   const int64_t n = rows * nb;
   if (ch <= 1) pack8_launch<E, 1>(s, x, ld, n, nb, D, codes, scales);
+  else if (ch <= 2) pack8_launch<E, 2>(s, x, ld, n, nb, D, codes, scales);
   else if (ch <= 4) pack8_launch<E, 4>(s, x, ld, n, nb, D, codes, scales);
+  else if (ch <= 8) pack8_launch<E, 8>(s, x, ld, n, nb, D, codes, scales);
   else pack8_launch<E, FULL>(s, x, ld, n, nb, D, codes, scales);
   return rs_status_after_launch();
 }

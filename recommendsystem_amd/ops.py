@@ -318,41 +318,38 @@ def _(ids, offsets, row_base, bucket, hash_mode, combiner, table):
 # sequence operators (sequence.py)
 # ============================================================================================
 @custom_op("ctr::layer_norm", mutates_args=())
-def layer_norm(x: Tensor, gamma: Tensor, beta: Tensor, epsilon: float) -> tuple[Tensor, Tensor, Tensor]:
-    """(y, mean, rstd) of sequence.layer_norm."""
+def layer_norm(x: Tensor, gamma: Tensor, beta: Tensor, epsilon: float) -> tuple[Tensor, Tensor]:
+    """sequence.layer_norm; returns (y, [means | 1 / standard deviations] [2, rows])."""
     code = sequence._check_norm(x, gamma, beta, epsilon)
     return _lib.run_on(_lib.device_index(x, gamma, beta), sequence._norm_forward, x, gamma, beta,
-                       epsilon, code, True, False)[:3]
+                       epsilon, code, True, False)[:2]
 
 
 @layer_norm.register_fake
 def _(x, gamma, beta, epsilon):
-    rows = x.numel() // x.shape[-1]
-    return (x.new_empty(x.shape), x.new_empty(rows, dtype=torch.float32),
-            x.new_empty(rows, dtype=torch.float32))
+    return x.new_empty(x.shape), gamma.new_empty(2, x.numel() // x.shape[-1])
 
 
 @custom_op("ctr::layer_norm_bwd", mutates_args=())
-def layer_norm_bwd(dy: Tensor, x: Tensor, gamma: Tensor, mean: Tensor,
-                   rstd: Tensor) -> tuple[Tensor, Tensor, Tensor]:
-    dx, dparams = _lib.run_on(_lib.device_index(dy, x, gamma, mean, rstd), sequence._norm_backward, dy,
-                              x, None, None, gamma, mean, rstd,
-                              packing.element_code(x, "layer_norm's input"), None, False)
-    return dx, dparams[0].clone(), dparams[1].clone()
+def layer_norm_bwd(dy: Tensor, x: Tensor, gamma: Tensor, stats: Tensor) -> tuple[Tensor, Tensor]:
+    """(dx, [dgamma | dbeta] [2, D])."""
+    return _lib.run_on(_lib.device_index(dy, x, gamma, stats), sequence._norm_backward, dy, x, None, None,
+                       gamma, stats, packing.element_code(x, "layer_norm's input"), None, False)
 
 
 @layer_norm_bwd.register_fake
-def _(dy, x, gamma, mean, rstd):
-    return dy.new_empty(dy.shape), torch.empty_like(gamma), torch.empty_like(gamma)
+def _(dy, x, gamma, stats):
+    return dy.new_empty(dy.shape), gamma.new_empty(2, gamma.shape[0])
 
 
 def _ln_setup(ctx, inputs, output):
     x, gamma, _, _ = inputs
-    ctx.save_for_backward(x, gamma, output[1], output[2])
+    ctx.save_for_backward(x, gamma, output[1])
 
 
-def _ln_backward(ctx, dy, _dmean, _drstd):
-    return (*torch.ops.ctr.layer_norm_bwd(dy, *ctx.saved_tensors), None)
+def _ln_backward(ctx, dy, _dstats):
+    dx, dparams = torch.ops.ctr.layer_norm_bwd(dy, *ctx.saved_tensors)
+    return dx, dparams[0], dparams[1], None
 
 
 layer_norm.register_autograd(_ln_backward, setup_context=_ln_setup)

@@ -62,9 +62,9 @@ def _check_norm(x, gamma, beta, epsilon):
                          f"{tuple(x.shape)}")
     D = x.shape[-1]
     for name, p in (("gamma", gamma), ("beta", beta)):
-        if p.dtype != torch.float32:
+        if p.dtype is not torch.float32:
             raise TypeError(f"layer_norm: {name} must be float32, got {p.dtype}")
-        if tuple(p.shape) != (D,):
+        if p.shape != (D,):
             raise ValueError(f"layer_norm: {name} {tuple(p.shape)} does not fit a last dimension of {D}")
     if not epsilon > 0:
         raise ValueError(f"layer_norm: epsilon must be positive, got {epsilon}")
@@ -75,31 +75,31 @@ def _norm_forward(x, gamma, beta, epsilon, code, stats, save_8bit, stream):
     x2 = rows_of(x)
     R, D = x2.shape
     y = x.new_empty(x.shape)
-    mean = rstd = codes = scales = None
+    mean = codes = scales = None  # mean: [means | 1 / standard deviations]
     if stats:
-        mean, rstd = gamma.new_empty(R), gamma.new_empty(R)
+        mean = gamma.new_empty((2, R))
     if save_8bit:
         codes = x.new_empty(x.shape, dtype=torch.int8)
         scales = gamma.new_empty(scale_shape(x.shape))
     call("rs_layernorm_fwd", stream, code, x2.data_ptr(), x2.stride(0), R, D,
          gamma.contiguous().data_ptr(), beta.contiguous().data_ptr(), epsilon, y.data_ptr(), D,
-         ptr(mean), ptr(rstd), ptr(codes), ptr(scales))
-    return y, mean, rstd, codes, scales
+         ptr(mean), mean.data_ptr() + 4 * R if stats else None, ptr(codes), ptr(scales))
+    return y, mean, codes, scales
 
 
-def _norm_backward(dy, x, codes, scales, gamma, mean, rstd, code, dparams, accumulate, stream):
+def _norm_backward(dy, x, codes, scales, gamma, mean, code, dparams, accumulate, stream):
     """dx; dparams: [dgamma | dbeta], made here where it is None."""
     dy2 = rows_of(dy)
     R, D = dy2.shape
     x2 = rows_of(x) if x is not None else None
     dx = dy.new_empty(dy.shape)
     if dparams is None:
-        dparams = gamma.new_empty(2, D)
+        dparams = gamma.new_empty((2, D))
     ws_n = _norm_workspace(R, D)
     ws = gamma.new_empty(ws_n)
     call("rs_layernorm_bwd", stream, code, dy2.data_ptr(), dy2.stride(0), ptr(x2),
          x2.stride(0) if x2 is not None else 0, ptr(codes), ptr(scales), R, D,
-         gamma.contiguous().data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), D,
+         gamma.contiguous().data_ptr(), mean.data_ptr(), mean.data_ptr() + 4 * R, dx.data_ptr(), D,
          dparams.data_ptr(), dparams.data_ptr() + 4 * D, accumulate, ws.data_ptr(), ws_n)
     return dx, dparams
 
@@ -110,19 +110,19 @@ class _LayerNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, gamma, beta, epsilon, code, save_8bit, in_place, index):
-        y, mean, rstd, codes, scales = run_on(index, _norm_forward, x, gamma, beta, epsilon, code,
-                                              True, save_8bit)
-        ctx.save_for_backward(None if save_8bit else x, codes, scales, gamma, beta, mean, rstd)
+        y, mean, codes, scales = run_on(index, _norm_forward, x, gamma, beta, epsilon, code, True,
+                                        save_8bit)
+        ctx.save_for_backward(None if save_8bit else x, codes, scales, gamma, beta, mean)
         ctx.args = code, in_place, index
         return y
 
     @_first_order
     def backward(ctx, dy):
-        x, codes, scales, gamma, beta, mean, rstd = ctx.saved_tensors
+        x, codes, scales, gamma, beta, mean = ctx.saved_tensors
         code, in_place, index = ctx.args
         block = grads_contiguous((gamma, beta)) if in_place else None
-        dx, dparams = run_on(index, _norm_backward, dy, x, codes, scales, gamma, mean, rstd, code,
-                             block, block is not None)
+        dx, dparams = run_on(index, _norm_backward, dy, x, codes, scales, gamma, mean, code, block,
+                             block is not None)
         dgamma, dbeta = dparams.unbind() if block is None else (None, None)
         return dx, dgamma, dbeta, None, None, None, None, None
 
@@ -180,11 +180,14 @@ class LayerNormalization(nn.Module):
 MAX_STEP_STRIDE = 2 ** 23  # elements between two steps (and of a step) that the kernels index
 
 
-def _unit(t):
-    """t [B, T, D] or [B, D] as the kernels read it: in place with unit stride along D and steps
-    not too far apart, a contiguous copy otherwise."""
-    unit = t.stride(-1) == 1 or t.shape[-1] == 1
-    return t if unit and (t.dim() < 3 or t.stride(1) < MAX_STEP_STRIDE) else t.contiguous()
+def _strided(t):
+    """t [B, T, D] as the kernels read it, and its batch and step strides: in place with unit stride
+    along D and steps not too far apart, a contiguous copy otherwise."""
+    sb, st, sc = t.stride()
+    if (sc != 1 and t.shape[2] != 1) or st >= MAX_STEP_STRIDE:
+        t = t.contiguous()
+        sb, st, sc = t.stride()
+    return t, sb, st
 
 
 def _halves(v, g):
@@ -225,23 +228,22 @@ def _any_grad(*tensors):
 def _check_state(state, shape, what):
     if state is None:
         return
-    if state.dtype != torch.float32:
+    if state.dtype is not torch.float32:
         raise TypeError(f"{what} must be float32, got {state.dtype}")
-    if tuple(state.shape) != shape:
+    if state.shape != shape:
         raise ValueError(f"{what} must be {shape}, got {tuple(state.shape)}")
 
 
 def _rec_forward(v, g, h0, lengths, code, keep, stream):
     v, g = _halves(v, g)
-    v, g = _unit(v), _unit(g)
     B, T, D = v.shape
+    v, v_sb, v_st = _strided(v)
+    g, g_sb, g_st = _strided(g)
     n_states, n_ws = _rec_sizes(code, B, T, D)
     h = v.new_empty((B, T, D))
     last = v.new_empty((B, D), dtype=torch.float32)
     states = last.new_empty(n_states) if keep else None
     ws = last.new_empty(n_ws) if n_ws else None
-    v_sb, v_st, _ = v.stride()
-    g_sb, g_st, _ = g.stride()
     call("rs_gated_rec_fwd", stream, code, v.data_ptr(), v_sb, v_st, g.data_ptr(), g_sb, g_st, B, T, D,
          ptr(lengths), ptr(h0), h.data_ptr(), last.data_ptr(), ptr(states), ptr(ws), n_ws)
     return h, last, states
@@ -250,24 +252,21 @@ def _rec_forward(v, g, h0, lengths, code, keep, stream):
 def _rec_backward(v, g, lengths, states, dh, dlast, code, want_h0, stream):
     """(dv, dg, dh0); with g None dv is the gradient of the joint rows and dg None."""
     joint = g is None
-    shape = v.shape
+    dvg = v.new_empty(v.shape)
+    dv, dg = _halves(dvg, None if joint else v.new_empty(v.shape))
     v, g = _halves(v, g)
-    v, g = _unit(v), _unit(g)
     B, T, D = v.shape
-    dvg = v.new_empty(shape)
-    dv, dg = _halves(dvg, None) if joint else (dvg, v.new_empty(shape))
-    dh0 = states.new_empty((B, D)) if want_h0 else None
+    v, v_sb, v_st = _strided(v)
+    g, g_sb, g_st = _strided(g)
+    d_sb, d_st, _ = dv.stride()
     dh_sb = dh_st = 0
     if dh is not None:
-        dh = _unit(dh)
-        dh_sb, dh_st, _ = dh.stride()
+        dh, dh_sb, dh_st = _strided(dh)
     if dlast is not None:
         dlast = dlast.contiguous()
+    dh0 = states.new_empty((B, D)) if want_h0 else None
     n_ws = _rec_sizes(code, B, T, D)[1]
     ws = states.new_empty(n_ws) if n_ws else None
-    v_sb, v_st, _ = v.stride()
-    g_sb, g_st, _ = g.stride()
-    d_sb, d_st, _ = dv.stride()
     call("rs_gated_rec_bwd", stream, code, v.data_ptr(), v_sb, v_st, g.data_ptr(), g_sb, g_st, B, T, D,
          ptr(lengths), states.data_ptr(), ptr(dh), dh_sb, dh_st, ptr(dlast), dv.data_ptr(), d_sb, d_st,
          dg.data_ptr(), d_sb, d_st, ptr(dh0), ptr(ws), n_ws)
@@ -349,7 +348,8 @@ def gated_recurrence_step(v, g=None, state=None, out=None):
 
 def _rec_step(v, g, state, out, B, D, code, stream):
     v, g = _halves(v, g)
-    v, g = _unit(v), _unit(g)
+    if D > 1:
+        v, g = (t if t.stride(1) == 1 else t.contiguous() for t in (v, g))
     if state is not None:
         state = state.contiguous()
     h = v.new_empty((B, D))

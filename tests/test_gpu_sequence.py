@@ -189,6 +189,9 @@ def test_layer_norm_offset_constant_and_not_finite():
     near(y, *want[0], "y")
     near(dx, *want[1], "dx")
     assert torch.equal(y[4], beta)
+    for D in (1, 7, 300, 5000, 20000):  # also where epsilon gives no slack at all
+        x, beta = torch.full((2, D), 0.1, device=DEV), rnd(D)
+        assert torch.equal(layer_norm(x, rnd(D), beta, 1e-14), beta.expand(2, D))
     # one row's NaN or infinity stays in that row
     x = rnd(5, 700)
     x[1, 3], x[3, 699] = float("nan"), float("inf")

@@ -115,10 +115,10 @@ def test_size_queries():
 def test_meta_shapes():
     m = dict(device="meta")
     x, p = E(4, 5, 300, dtype=BF16, **m), E(300, **m)
-    y, mean, rstd = torch.ops.ctr.layer_norm(x, p, p, 1e-5)
-    assert y.shape == x.shape and y.dtype == BF16 and mean.shape == rstd.shape == (20,)
-    dx, dg, db = torch.ops.ctr.layer_norm_bwd(y, x, p, mean, rstd)
-    assert dx.shape == x.shape and dg.shape == db.shape == (300,) and dg.dtype == F32
+    y, stats = torch.ops.ctr.layer_norm(x, p, p, 1e-5)
+    assert y.shape == x.shape and y.dtype == BF16 and stats.shape == (2, 20)
+    dx, dparams = torch.ops.ctr.layer_norm_bwd(y, x, p, stats)
+    assert dx.shape == x.shape and dparams.shape == (2, 300) and dparams.dtype == F32
     h, last, states = torch.ops.ctr.gated_recurrence(x, None, None, None)
     assert h.shape == (4, 5, 150) and last.shape == (4, 150) and last.dtype == F32
     dv, dgt, dh0 = torch.ops.ctr.gated_recurrence_bwd(h, last, x, None, None, states)
