@@ -890,8 +890,8 @@ int rs_layernorm_bwd(void* stream, int dtype, const void* dy, int64_t ld_dy, con
  * taken into 0..T): steps behind them are not read, h is zero there and the state stands still.
  * D and step strides (*_st) of 2^23 elements or more: -2.
  * h [B, T, D] contiguous; last [B, D]: the state after lengths[b] steps.  states
- * (rs_gated_rec_states_floats; NULL without a backward): fp32 states at fixed steps, for
- * rs_gated_rec_bwd with the same shape.  workspace: rs_gated_rec_workspace_floats floats. */
+ * (rs_gated_rec_states_floats, 0 for short sequences; NULL without a backward): fp32 states at
+ * fixed steps, for rs_gated_rec_bwd with the same shape.  workspace: rs_gated_rec_workspace_floats floats. */
 int64_t rs_gated_rec_states_floats(int dtype, int64_t B, int64_t T, int D);
 int64_t rs_gated_rec_workspace_floats(int dtype, int64_t B, int64_t T, int D);
 int rs_gated_rec_fwd(void* stream, int dtype, const void* v, int64_t v_sb, int64_t v_st,
@@ -899,11 +899,11 @@ int rs_gated_rec_fwd(void* stream, int dtype, const void* v, int64_t v_sb, int64
                      const int32_t* lengths, const float* h0, void* h, float* last, float* states,
                      float* workspace, int64_t workspace_floats);
 /* dv, dg [B, T, D] (strided, zero behind lengths; the halves of one [B, T, 2 D] buffer, say), dh0
- * [B, D] (nullable) from dh [B, T, D] (NULL: zeros) and dlast [B, D] (NULL: zeros). */
+ * [B, D] (nullable) from dh [B, T, D] (NULL: zeros) and dlast [B, D] (NULL: zeros); h0 is the forward's. */
 int rs_gated_rec_bwd(void* stream, int dtype, const void* v, int64_t v_sb, int64_t v_st,
                      const void* g, int64_t g_sb, int64_t g_st, int64_t B, int64_t T, int D,
-                     const int32_t* lengths, const float* states, const void* dh, int64_t dh_sb,
-                     int64_t dh_st, const float* dlast, void* dv, int64_t dv_sb, int64_t dv_st,
+                     const int32_t* lengths, const float* h0, const float* states, const void* dh,
+                     int64_t dh_sb, int64_t dh_st, const float* dlast, void* dv, int64_t dv_sb, int64_t dv_st,
                      void* dg, int64_t dg_sb, int64_t dg_st, float* dh0, float* workspace,
                      int64_t workspace_floats);
 /* One step for B tokens: v, g [B, D] (row strides ld_*), state [B, D] fp32 (NULL: zeros) ->

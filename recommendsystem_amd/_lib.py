@@ -114,7 +114,7 @@ SIGNATURES: dict[str, tuple] = {
     "rs_gated_rec_fwd": (_i32, [_vp, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp,
                                 _vp, _vp, _vp, _vp, _vp, _i64]),
     "rs_gated_rec_bwd": (_i32, [_vp, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp,
-                                _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                                _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
                                 _i64]),
     "rs_gated_rec_step": (_i32, [_vp, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
     "rs_din_param_count": (_i32, [_i32, _i32]),

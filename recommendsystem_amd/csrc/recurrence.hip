@@ -15,7 +15,7 @@
 // in flight.  So everything is read once and written once, whatever the length.
 //
 // The backward computes the states again from v and g, tile by tile, from the fp32 states that
-// the forward kept in front of every tile; h itself (rounded to the rows' type) is not used.
+// the forward kept in front of every tile (of a sequence in one tile that is h0); h itself (rounded to the rows' type) is not used.
 //
 // Where B and D give too few workgroups to fill the chip, the time axis is cut into segments: a
 // first launch reduces every segment to its (A, H), and each workgroup of the second folds those in
@@ -553,6 +553,8 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
 
   Half nv_[K], ng_[K], nd_[K];
   float ns[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) ns[j] = 0.f;
   auto load_as = [&](int tile, auto whole) __attribute__((always_inline)) {
     const int64_t t = wave_step<LC, NG, K>(tile);
 #pragma unroll
@@ -563,7 +565,8 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
       load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, some), p.nv, in, 0u);
       load8<E, PART>(nd_[k], W ? rd_.at(t, k) : rd_.in(t, k, some), p.nv, in && !none, 0u);
     }
-    load_n<V>(ns, a.states + (p.b * a.tiles + tile) * a.D + p.c0, p.nv);
+    if (a.states) load_n<V>(ns, a.states + (p.b * a.tiles + tile) * a.D + p.c0, p.nv);
+    else if (a.h0) load_n<V>(ns, a.h0 + ch, p.nv);  // one tile
   };
   auto load = [&](int tile) __attribute__((always_inline)) {
     if (NG > 1 && (int64_t)(tile + 1) * STEPS <= p.n) load_as(tile, Yes());
@@ -666,17 +669,25 @@ __global__ void __launch_bounds__(256) rec_step_kernel(const RecArgs a, float* n
 // ---------------------------------------------------------------------------------------------
 namespace {
 
-constexpr int REC_LC = 16;  // lanes to a row of a channel tile: 128 bytes
-//   FLAT   T <= 8: a thread per 8 bytes of channels, nothing to join
-//   WAVE   tiles of 64 steps on 128 threads: T <= 64, or workgroups enough without more threads each
-//          (forward + backward us, bf16, D = 2048, WAVE / BLOCK: 64 x 512 steps, 2048 workgroups, 258 /
-//          288; 128 x 256 steps, 4096, 228 / 274; 24 x 2048 steps, 768, 371 / 357; 8 x 4096 steps, 256,
-//          401 / 266)
-//   BLOCK  tiles of 256 steps on 512 threads, one workgroup a compute unit.  Up to 128 workgroups
-//          the time axis is cut so that there are at most 256, one round (65521 x 1000 fp16 forward:
-//          133 us with 16 segments, 151 with 32 in two rounds); above 128 a cut would read the input
-//          twice to fill less than half of the chip more.
-enum { REC_FLAT, REC_WAVE, REC_BLOCK };
+//   FLAT  tiles of 8 steps, a thread per 8 bytes of channels, nothing to join: T <= 8, or rows that
+//         fill no more than a quarter of the other kinds' tiles, and enough of them
+//   SHORT T <= 32: tiles of 32 steps x 128 bytes of channels, one wave
+//   WAVE  tiles of 64 steps x 128 bytes of channels, 128 threads, several workgroups a compute unit:
+//         short sequences, or middling ones of many workgroups, whose first loads then overlap
+//   LONG  256 steps x 128 bytes, 512 threads, one workgroup a compute unit
+//   WIDE  128 steps x 256 bytes, 512 threads: rows are read in longer pieces, which memory likes, but
+//         it takes twice the channels for as many workgroups
+// Forward + backward, us, bf16 (number of 128-byte tiles):        WAVE   LONG   WIDE
+//   1024 x   50 x 1024 (16384)                                     203    810    419
+//    256 x  256 x 1024 (4096)                                      225    270    269
+//     64 x 1024 x 2048 (2048)                                      486    482    446
+//     12 x 4096 x 2048 (384)                                       510    431    410
+//      8 x 4096 x 2048 (256)                                       400    268    302
+//     37 x  300 x  333 (222)                                        78     45     94
+// Up to 128 workgroups the time axis is cut so that there are at most 256, one round (65521 x 1000
+// fp16 forward: 133 us with 16 segments, 151 with 32 in two rounds); above 128 a cut would read the
+// input twice to fill less than half of the chip more.
+enum { REC_FLAT, REC_SHORT, REC_WAVE, REC_LONG, REC_WIDE };
 struct RecPlan {
   int kind, steps;  // steps: of a time tile
   int nct, segs, tps;
@@ -685,15 +696,26 @@ struct RecPlan {
 
 RecPlan rec_plan(int dtype, int64_t B, int64_t T, int D) {
   const int V = dtype == RS_F32 ? 2 : 4;
+  const int n16 = (D + 16 * V - 1) / (16 * V), n32 = (n16 + 1) / 2;  // channel tiles
+  const int64_t b16 = B * n16, b32 = B * n32;
+  // (a cut sequence has workgroups enough either way: wide tiles unless much of them lies beyond D)
+  const bool wide = b32 >= 160 || (b16 <= 128 && n16 >= 8);
   RecPlan p;
-  p.nct = (D + REC_LC * V - 1) / (REC_LC * V);
-  const int64_t blocks = B * p.nct;
-  p.kind = T <= 8 ? REC_FLAT : T <= 64 || blocks >= 1024 ? REC_WAVE : REC_BLOCK;
-  p.steps = p.kind == REC_FLAT ? 8 : p.kind == REC_WAVE ? 64 : 256;
+  const bool narrow = 4 * D <= 16 * V && T <= 512 && B * ((D + V - 1) / V) >= 65536;
+  p.kind = T <= 8 || narrow                  ? REC_FLAT
+           : T <= 32                         ? REC_SHORT
+           : T <= 64                         ? REC_WAVE
+           : T <= 512 && b16 >= 512          ? REC_WAVE
+           : wide                            ? REC_WIDE
+                                             : REC_LONG;
+  constexpr int STEPS[] = {8, 32, 64, 256, 128};  // by kind
+  p.steps = STEPS[p.kind];
+  p.nct = p.kind == REC_WIDE ? n32 : n16;
   p.tiles = (T + p.steps - 1) / p.steps;
   p.segs = 1;
   p.tps = (int)p.tiles;
-  if (p.kind == REC_BLOCK && blocks <= 128 && p.tiles > 1) {
+  const int64_t blocks = B * p.nct;
+  if ((p.kind == REC_LONG || p.kind == REC_WIDE) && blocks <= 128 && p.tiles > 1) {
     const int64_t want = 256 / blocks;
     p.tps = (int)((p.tiles + want - 1) / want);
     p.segs = (int)((p.tiles + p.tps - 1) / p.tps);
@@ -717,11 +739,16 @@ int rec_fwd_as(hipStream_t s, const RecPlan& p, const RecArgs& a) {
   if (p.kind == REC_FLAT) {
     const int64_t n = a.B * ((a.D + VC<E>::V - 1) / VC<E>::V);
     rec_fwd_kernel<E, 64, 1, 8, PART><<<(unsigned)((n + 63) / 64), 64, 0, s>>>(a);
+  } else if (p.kind == REC_SHORT) {
+    rec_fwd_kernel<E, 16, 4, 8, PART><<<per, 64, 0, s>>>(a);
   } else if (p.kind == REC_WAVE) {
-    rec_fwd_kernel<E, REC_LC, 8, 8, PART><<<per, 128, 0, s>>>(a);
+    rec_fwd_kernel<E, 16, 8, 8, PART><<<per, 128, 0, s>>>(a);
+  } else if (p.kind == REC_LONG) {
+    if (p.segs > 1) rec_sum_kernel<E, 16, 32, 8, true, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
+    rec_fwd_kernel<E, 16, 32, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
   } else {
-    if (p.segs > 1) rec_sum_kernel<E, REC_LC, 32, 8, true, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
-    rec_fwd_kernel<E, REC_LC, 32, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
+    if (p.segs > 1) rec_sum_kernel<E, 32, 16, 8, true, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
+    rec_fwd_kernel<E, 32, 16, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
   }
   return rs_status_after_launch();
 }
@@ -732,11 +759,16 @@ int rec_bwd_as(hipStream_t s, const RecPlan& p, const RecArgs& a) {
   if (p.kind == REC_FLAT) {
     const int64_t n = a.B * ((a.D + VC<E>::V - 1) / VC<E>::V);
     rec_bwd_kernel<E, 64, 1, 8, PART><<<(unsigned)((n + 63) / 64), 64, 0, s>>>(a);
+  } else if (p.kind == REC_SHORT) {
+    rec_bwd_kernel<E, 16, 4, 8, PART><<<per, 64, 0, s>>>(a);
   } else if (p.kind == REC_WAVE) {
-    rec_bwd_kernel<E, REC_LC, 8, 8, PART><<<per, 128, 0, s>>>(a);
+    rec_bwd_kernel<E, 16, 8, 8, PART><<<per, 128, 0, s>>>(a);
+  } else if (p.kind == REC_LONG) {
+    if (p.segs > 1) rec_sum_kernel<E, 16, 32, 8, false, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
+    rec_bwd_kernel<E, 16, 32, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
   } else {
-    if (p.segs > 1) rec_sum_kernel<E, REC_LC, 32, 8, false, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
-    rec_bwd_kernel<E, REC_LC, 32, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
+    if (p.segs > 1) rec_sum_kernel<E, 32, 16, 8, false, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
+    rec_bwd_kernel<E, 32, 16, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
   }
   return rs_status_after_launch();
 }
@@ -772,7 +804,8 @@ bool rec_shape_ok(int dtype, int64_t B, int64_t T, int D) {
 
 RS_API int64_t rs_gated_rec_states_floats(int dtype, int64_t B, int64_t T, int D) {
   if (!rec_shape_ok(dtype, B, T, D)) return 0;
-  return B * rec_plan(dtype, B, T, D).tiles * D;
+  const int64_t tiles = rec_plan(dtype, B, T, D).tiles;
+  return tiles > 1 ? B * tiles * D : 0;
 }
 
 RS_API int64_t rs_gated_rec_workspace_floats(int dtype, int64_t B, int64_t T, int D) {
@@ -797,23 +830,26 @@ RS_API int rs_gated_rec_fwd(void* stream, int dtype, const void* v, int64_t v_sb
   rec_fill(a, p, B, T, D);
   a.v = v, a.v_sb = v_sb, a.v_st = v_st;
   a.g = g, a.g_sb = g_sb, a.g_st = g_st;
-  a.lengths = lengths, a.h0 = h0, a.h = h, a.last = last, a.states = states, a.ws = workspace;
+  a.lengths = lengths, a.h0 = h0, a.h = h, a.last = last, a.ws = workspace;
+  a.states = p.tiles > 1 ? states : nullptr;
   return RS_DISPATCH_ELEM(dtype, rec_fwd, rs_stream(stream), p, a);
 }
 
 RS_API int rs_gated_rec_bwd(void* stream, int dtype, const void* v, int64_t v_sb, int64_t v_st,
                             const void* g, int64_t g_sb, int64_t g_st, int64_t B, int64_t T, int D,
-                            const int32_t* lengths, const float* states, const void* dh,
-                            int64_t dh_sb, int64_t dh_st, const float* dlast, void* dv,
+                            const int32_t* lengths, const float* h0, const float* states,
+                            const void* dh, int64_t dh_sb, int64_t dh_st, const float* dlast, void* dv,
                             int64_t dv_sb, int64_t dv_st, void* dg, int64_t dg_sb, int64_t dg_st,
                             float* dh0, float* workspace, int64_t workspace_floats) {
   if (!rec_shape_ok(dtype, B, T, D)) return RS_ERR_ARG;
   if (B == 0) return RS_OK;
-  if (T > 0 && (!v || !g || !states || !dv || !dg || v_sb < 0 || v_st < 0 || g_sb < 0 ||
+  if (T > 0 && (!v || !g || !dv || !dg || v_sb < 0 || v_st < 0 || g_sb < 0 ||
                 g_st < 0 || dh_sb < 0 || dh_st < 0 || (T > 1 && (dv_st < D || dg_st < D)) ||
                 (B > 1 && (dv_sb < D || dg_sb < D))))
     return RS_ERR_ARG;
   if (T == 0 && !dh0) return RS_OK;
+  const bool kept = rs_gated_rec_states_floats(dtype, B, T, D) > 0;
+  if (kept && !states) return RS_ERR_ARG;
   if (!rec_strides_ok(v_st, g_st, dh_st) || !rec_strides_ok(dv_st, dg_st, D)) return RS_ERR_UNSUPPORTED;
   const int64_t need = rs_gated_rec_workspace_floats(dtype, B, T, D);
   if (need > 0 && (!workspace || workspace_floats < need)) return RS_ERR_ARG;
@@ -823,7 +859,8 @@ RS_API int rs_gated_rec_bwd(void* stream, int dtype, const void* v, int64_t v_sb
   a.v = v, a.v_sb = v_sb, a.v_st = v_st;
   a.g = g, a.g_sb = g_sb, a.g_st = g_st;
   a.dh = dh, a.dh_sb = dh_sb, a.dh_st = dh_st;
-  a.lengths = lengths, a.states = const_cast<float*>(states), a.dlast = dlast;
+  a.lengths = lengths, a.states = kept ? const_cast<float*>(states) : nullptr, a.h0 = h0;
+  a.dlast = dlast;
   a.dv = dv, a.dv_sb = dv_sb, a.dv_st = dv_st;
   a.dg = dg, a.dg_sb = dg_sb, a.dg_st = dg_st;
   a.dh0 = dh0, a.ws = workspace;

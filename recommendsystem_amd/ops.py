@@ -366,9 +366,10 @@ def gated_recurrence(v: Tensor, g: Optional[Tensor], h0: Optional[Tensor],
     code = sequence._check_rec(v, g, 3, "gated_recurrence")
     B, T, D = _rec_sizes(v, g)
     sequence._check_state(h0, (B, D), "gated_recurrence: h0")
-    return _lib.run_on(_lib.device_index(v, g, h0, lengths), sequence._rec_forward, v, g,
-                       h0.contiguous() if h0 is not None else None,
-                       sequence._check_lengths(lengths, B, T), code, True)
+    h, last, states = _lib.run_on(_lib.device_index(v, g, h0, lengths), sequence._rec_forward, v, g,
+                                  h0.contiguous() if h0 is not None else None,
+                                  sequence._check_lengths(lengths, B, T), code, True)
+    return h, last, last.new_empty(0) if states is None else states
 
 
 @gated_recurrence.register_fake
@@ -382,31 +383,32 @@ def _(v, g, h0, lengths):
 
 @custom_op("ctr::gated_recurrence_bwd", mutates_args=())
 def gated_recurrence_bwd(dh: Tensor, dlast: Tensor, v: Tensor, g: Optional[Tensor],
-                         lengths: Optional[Tensor], states: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+                         h0: Optional[Tensor], lengths: Optional[Tensor], states: Tensor) -> tuple[Tensor, Tensor, Tensor]:
     """(dv, dg, dh0); with g None dv is the joint rows' gradient and dg is empty."""
     B, T, D = _rec_sizes(v, g)
-    dv, dg, dh0 = _lib.run_on(_lib.device_index(v, g, dh, dlast, lengths, states),
-                              sequence._rec_backward, v, g, sequence._check_lengths(lengths, B, T),
-                              states, dh, dlast, packing.element_code(v, "gated_recurrence's values"),
+    dv, dg, dh0 = _lib.run_on(_lib.device_index(v, g, dh, dlast, h0, lengths, states),
+                              sequence._rec_backward, v, g,
+                              h0.contiguous() if h0 is not None else None,
+                              sequence._check_lengths(lengths, B, T), states, dh, dlast, packing.element_code(v, "gated_recurrence's values"),
                               True)
     return dv, v.new_empty(0) if dg is None else dg, dh0
 
 
 @gated_recurrence_bwd.register_fake
-def _(dh, dlast, v, g, lengths, states):
+def _(dh, dlast, v, g, h0, lengths, states):
     return (v.new_empty(v.shape), v.new_empty(0) if g is None else v.new_empty(v.shape),
             torch.empty_like(dlast))
 
 
 def _rec_setup(ctx, inputs, output):
     v, g, h0, lengths = inputs
-    ctx.save_for_backward(v, g, lengths, output[2])
+    ctx.save_for_backward(v, g, h0, lengths, output[2])
     ctx.has_g, ctx.has_h0 = g is not None, h0 is not None
 
 
 def _rec_op_backward(ctx, dh, dlast, _dstates):
-    v, g, lengths, states = ctx.saved_tensors
-    dv, dg, dh0 = torch.ops.ctr.gated_recurrence_bwd(dh, dlast, v, g, lengths, states)
+    v, g, h0, lengths, states = ctx.saved_tensors
+    dv, dg, dh0 = torch.ops.ctr.gated_recurrence_bwd(dh, dlast, v, g, h0, lengths, states)
     return dv, dg if ctx.has_g else None, dh0 if ctx.has_h0 else None, None
 
 

@@ -242,14 +242,14 @@ def _rec_forward(v, g, h0, lengths, code, keep, stream):
     n_states, n_ws = _rec_sizes(code, B, T, D)
     h = v.new_empty((B, T, D))
     last = v.new_empty((B, D), dtype=torch.float32)
-    states = last.new_empty(n_states) if keep else None
+    states = last.new_empty(n_states) if keep and n_states else None
     ws = last.new_empty(n_ws) if n_ws else None
     call("rs_gated_rec_fwd", stream, code, v.data_ptr(), v_sb, v_st, g.data_ptr(), g_sb, g_st, B, T, D,
          ptr(lengths), ptr(h0), h.data_ptr(), last.data_ptr(), ptr(states), ptr(ws), n_ws)
     return h, last, states
 
 
-def _rec_backward(v, g, lengths, states, dh, dlast, code, want_h0, stream):
+def _rec_backward(v, g, h0, lengths, states, dh, dlast, code, want_h0, stream):
     """(dv, dg, dh0); with g None dv is the gradient of the joint rows and dg None."""
     joint = g is None
     dvg = v.new_empty(v.shape)
@@ -264,11 +264,11 @@ def _rec_backward(v, g, lengths, states, dh, dlast, code, want_h0, stream):
         dh, dh_sb, dh_st = _strided(dh)
     if dlast is not None:
         dlast = dlast.contiguous()
-    dh0 = states.new_empty((B, D)) if want_h0 else None
+    dh0 = v.new_empty((B, D), dtype=torch.float32) if want_h0 else None
     n_ws = _rec_sizes(code, B, T, D)[1]
-    ws = states.new_empty(n_ws) if n_ws else None
+    ws = v.new_empty(n_ws, dtype=torch.float32) if n_ws else None
     call("rs_gated_rec_bwd", stream, code, v.data_ptr(), v_sb, v_st, g.data_ptr(), g_sb, g_st, B, T, D,
-         ptr(lengths), states.data_ptr(), ptr(dh), dh_sb, dh_st, ptr(dlast), dv.data_ptr(), d_sb, d_st,
+         ptr(lengths), ptr(h0), ptr(states), ptr(dh), dh_sb, dh_st, ptr(dlast), dv.data_ptr(), d_sb, d_st,
          dg.data_ptr(), d_sb, d_st, ptr(dh0), ptr(ws), n_ws)
     return dvg, None if joint else dg, dh0
 
@@ -278,17 +278,17 @@ class _RecurrenceFn(torch.autograd.Function):
     def forward(ctx, v, g, h0, lengths, code, index):
         ctx.set_materialize_grads(False)
         h, last, states = run_on(index, _rec_forward, v, g, h0, lengths, code, True)
-        ctx.save_for_backward(v, g, lengths, states)
+        ctx.save_for_backward(v, g, h0, lengths, states)
         ctx.args = code, index
         return h, last
 
     @_first_order
     def backward(ctx, dh, dlast):
-        v, g, lengths, states = ctx.saved_tensors
+        v, g, h0, lengths, states = ctx.saved_tensors
         if dh is None and dlast is None:
             return None, None, None, None, None, None
         code, index = ctx.args
-        return (*run_on(index, _rec_backward, v, g, lengths, states, dh, dlast, code,
+        return (*run_on(index, _rec_backward, v, g, h0, lengths, states, dh, dlast, code,
                         ctx.needs_input_grad[2]), None, None, None)
 
 

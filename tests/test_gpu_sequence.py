@@ -303,7 +303,8 @@ def ref_rec(v, g, h0, lengths, dh=None, dlast=None):
 
 REC_SHAPES = [(1, 1, 1), (3, 1, 40), (2, 2, 7), (1, 3, 8), (5, 7, 5), (2, 8, 64), (3, 9, 65), (2, 16, 33), (4, 50, 32),
               (3, 63, 8), (2, 64, 130), (2, 65, 9), (1, 127, 72), (2, 128, 8), (1, 255, 40), (2, 256, 16), (1, 257, 136),
-              (1, 500, 24), (2, 513, 64), (1, 1023, 8), (1, 1030, 264), (1, 2500, 4), (300, 20, 16), (70, 100, 48)]
+              (1, 500, 24), (2, 513, 64), (1, 1023, 8), (1, 1030, 264), (1, 2500, 4), (300, 20, 16), (70, 100, 48), (170, 130, 130),
+              (1, 1500, 515), (3, 700, 1030), (170, 65, 264), (17000, 11, 16)]
 
 
 @pytest.mark.parametrize("ragged", [False, True], ids=["", "ragged"])

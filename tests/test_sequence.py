@@ -92,8 +92,8 @@ def test_entry_points_reject():
     assert lib.rs_gated_rec_fwd(None, 0, p, 4, 4, p, 4, 4, 1, -1, 4, None, None, p, p, None, None, 0) == ARG
     assert lib.rs_gated_rec_fwd(None, 0, p, 4, 4, p, 4, 4, 1, 1, 4, None, None, p, None, None, None, 0) == ARG
     assert lib.rs_gated_rec_fwd(None, 0, p, 4, 4, p, 4, 4, 0, 9, 4, None, None, None, None, None, None, 0) == 0
-    assert lib.rs_gated_rec_bwd(None, 0, p, 4, 4, p, 4, 4, 1, 1, 4, None, None, p, 4, 4, p, p, 4, 4, p, 4, 4,
-                                p, None, 0) == ARG                   # no states
+    assert lib.rs_gated_rec_bwd(None, 0, p, 4, 4, p, 4, 4, 1, 999, 4, None, None, None, p, 4, 4, p, p, 4, 4, p,
+                                4, 4, p, None, 0) == ARG             # no states
     assert lib.rs_gated_rec_step(None, 0, p, 4, p, 4, 1, 4, p, p, None) == ARG
     # a workspace that the shape needs and that is missing
     B, T, D = 1, 1 << 20, 8
@@ -121,7 +121,7 @@ def test_meta_shapes():
     assert dx.shape == x.shape and dparams.shape == (2, 300) and dparams.dtype == F32
     h, last, states = torch.ops.ctr.gated_recurrence(x, None, None, None)
     assert h.shape == (4, 5, 150) and last.shape == (4, 150) and last.dtype == F32
-    dv, dgt, dh0 = torch.ops.ctr.gated_recurrence_bwd(h, last, x, None, None, states)
+    dv, dgt, dh0 = torch.ops.ctr.gated_recurrence_bwd(h, last, x, None, None, None, states)
     assert dv.shape == x.shape and dgt.numel() == 0 and dh0.shape == (4, 150)
     codes, scales = torch.ops.ctr.pack8(x)
     assert codes.shape == x.shape and codes.dtype == torch.int8 and scales.shape == (4, 5, 3)
