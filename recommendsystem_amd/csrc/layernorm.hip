@@ -470,47 +470,63 @@ __global__ void __launch_bounds__(64) ln_wide_params_kernel(const LnArgs a) {
 // ---------------------------------------------------------------------------------------------
 namespace {
 
-// (threads of a row, 16-byte pieces a thread), the first that holds the row: at most a third of the
-// lanes without work.  Few threads with several pieces rather than many with one: fewer exchanges.
-#define LN_SHAPES(X)                                                                            \
-  X(1, 1) X(1, 2) X(1, 3) X(2, 2) X(2, 3) X(4, 2) X(4, 3) X(8, 2) X(8, 3) X(16, 2) X(16, 3)     \
-  X(32, 2) X(32, 3) X(64, 2) X(64, 3) X(64, 4) X(128, 3) X(128, 4) X(256, 3) X(256, 4)          \
-  X(512, 3) X(512, 4)
+// X(threads of a row, 16-byte pieces a thread, pieces from, pieces to): the first that holds the row,
+// with at most a third of the lanes without work.  A power of two of pieces takes a lane each up to a
+// wave (131072 x 256 fp32, forward + backward: 127 us, half the lanes with two pieces 147 us), other
+// widths few lanes with several (200000 x 100 bf16: 60 us, 16 lanes with one piece 76 us).
+#define LN_SHAPES(X)                                                                              \
+  X(1, 1, 1, 1) X(4, 1, 4, 4) X(8, 1, 8, 8) X(16, 1, 16, 16) X(32, 1, 32, 32) X(64, 1, 64, 64)    \
+  X(1, 2, 1, 2) X(1, 3, 1, 3) X(2, 3, 1, 6) X(4, 2, 1, 8) X(4, 3, 1, 12) X(8, 2, 1, 16)           \
+  X(8, 3, 1, 24) X(16, 2, 1, 32) X(16, 3, 1, 48) X(32, 2, 1, 64) X(32, 3, 1, 96)                  \
+  X(64, 2, 1, 128) X(64, 3, 1, 192) X(64, 4, 1, 256) X(128, 3, 1, 384) X(128, 4, 1, 512)          \
+  X(256, 3, 1, 768) X(256, 4, 1, 1024) X(512, 3, 1, 1536) X(512, 4, 1, 2048)
 
 int ln_pieces(int D, int V) { return (D + V - 1) / V; }
 
-int ln_tpr(int pieces) {
-#define LN_TPR(TPR, NCH) \
-  if (pieces <= TPR * NCH) return TPR;
-  LN_SHAPES(LN_TPR)
-#undef LN_TPR
-  return 0;  // wider
+struct LnPlan {
+  int tpr, nch;  // 0: wider than any shape
+};
+LnPlan ln_plan(int pieces) {
+#define LN_PLAN(TPR, NCH, FROM, TO) \
+  if (pieces >= FROM && pieces <= TO) return {TPR, NCH};
+  LN_SHAPES(LN_PLAN)
+#undef LN_PLAN
+  return {0, 0};
 }
 
+int64_t ln_rounds(int64_t rows, int tpr) {  // of one workgroup over all rows
+  const int64_t rpb = tpr < 256 ? 256 / tpr : 1;
+  return (rows + rpb - 1) / rpb;
+}
 int64_t ln_grid(int64_t rows, int tpr, int64_t most) {
-  const int64_t rpb = tpr < 256 ? 256 / tpr : 1, n = (rows + rpb - 1) / rpb;
+  const int64_t n = ln_rounds(rows, tpr);
   return n < most ? n : most;
 }
 
-// partial rows of the parameters' gradients: two workgroups a compute unit, which is what the
-// backward's registers allow; for wider rows as many groups of rows as give 1024 or so waves
+// Partial rows of the parameters' gradients = workgroups of the backward: two a compute unit, which
+// is what its registers allow with 32 elements a thread, and more of them measured slower down to 8
+// elements (65536 x 1024 bf16: 78 us, with 1024 workgroups 95; 400000 x 64 bf16: 34 us, with 2048 38).
+// Narrow rows of 4 elements a thread have too few bytes in flight so (400000 x 64 fp32: 90 us, with
+// 2048 63).  For rows wider than any shape, as many groups of rows as give 1024 waves or so.
 int64_t ln_parts(int64_t rows, int D, int V) {
-  const int tpr = ln_tpr(ln_pieces(D, V));
-  if (tpr) return ln_grid(rows, tpr, 512);
-  const int64_t most = 65536 / ln_pieces(D, V) + 1;
-  return rows < most ? rows : most;
+  const LnPlan p = ln_plan(ln_pieces(D, V));
+  if (!p.tpr) {
+    const int64_t most = 65536 / ln_pieces(D, V) + 1;
+    return rows < most ? rows : most;
+  }
+  return ln_grid(rows, p.tpr, p.nch * V <= 4 && D <= 128 ? 2048 : 512);
 }
 
 template <class E>
 int ln_fwd(hipStream_t s, const LnArgs& a) {
-  const int pieces = ln_pieces(a.D, E::V), tpr = ln_tpr(pieces);
+  const int pieces = ln_pieces(a.D, E::V), tpr = ln_plan(pieces).tpr;
   if (!tpr) {
     ln_wide_fwd_kernel<E><<<(unsigned)(a.rows < 65536 ? a.rows : 65536), LN_WIDE, 0, s>>>(a);
     return rs_status_after_launch();
   }
   const unsigned grid = (unsigned)ln_grid(a.rows, tpr, 2048);
-#define LN_FWD(TPR, NCH)                                                               \
-  if (pieces <= TPR * NCH) {                                                           \
+#define LN_FWD(TPR, NCH, FROM, TO)                                                     \
+  if (pieces >= FROM && pieces <= TO) {                                                \
     if (a.codes) ln_fwd_kernel<E, TPR, NCH, true><<<grid, LnShape<TPR>::THREADS, 0, s>>>(a); \
     else ln_fwd_kernel<E, TPR, NCH, false><<<grid, LnShape<TPR>::THREADS, 0, s>>>(a);  \
     return rs_status_after_launch();                                                   \
@@ -523,8 +539,8 @@ int ln_fwd(hipStream_t s, const LnArgs& a) {
 template <class E>
 void ln_bwd_rows(hipStream_t s, const LnArgs& a, unsigned grid) {
   const int pieces = ln_pieces(a.D, E::V);
-#define LN_BWD(TPR, NCH)                                                               \
-  if (pieces <= TPR * NCH) {                                                           \
+#define LN_BWD(TPR, NCH, FROM, TO)                                                     \
+  if (pieces >= FROM && pieces <= TO) {                                                \
     if (a.codes) ln_bwd_kernel<E, TPR, NCH, true><<<grid, LnShape<TPR>::THREADS, 0, s>>>(a); \
     else ln_bwd_kernel<E, TPR, NCH, false><<<grid, LnShape<TPR>::THREADS, 0, s>>>(a);  \
     return;                                                                            \
@@ -535,7 +551,7 @@ void ln_bwd_rows(hipStream_t s, const LnArgs& a, unsigned grid) {
 
 template <class E>
 int ln_bwd(hipStream_t s, const LnArgs& a) {
-  const bool wide = !ln_tpr(ln_pieces(a.D, E::V));
+  const bool wide = !ln_plan(ln_pieces(a.D, E::V)).tpr;
   const unsigned parts = (unsigned)ln_parts(a.rows, a.D, E::V);
   if (a.rows && wide) {
     const unsigned grid = (unsigned)(a.rows < 65536 ? a.rows : 65536);
@@ -576,7 +592,7 @@ RS_API int64_t rs_layernorm_bwd_workspace_floats(int64_t rows, int D) {
   if (rows < 0 || D <= 0 || D > LN_MAX_D) return 0;
   int64_t most = 0;
   for (int V = 4; V <= 8; V += 4) {
-    const int64_t n = ln_parts(rows, D, V) * 2 * D + (ln_tpr(ln_pieces(D, V)) ? 0 : rows);
+    const int64_t n = ln_parts(rows, D, V) * 2 * D + (ln_plan(ln_pieces(D, V)).tpr ? 0 : rows);
     if (n > most) most = n;
   }
   return most;
