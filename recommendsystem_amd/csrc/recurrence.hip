@@ -416,8 +416,10 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
     if (NG > 1 && (int64_t)(tile + 1) * STEPS <= p.n) load_as(tile, Yes());
     else load_as(tile, No());
   };
-  if (t1 > t0) load(t0);
-  for (int tile = t0; tile < t1; ++tile) {
+  // tiles wholly behind the sequence's end: nothing to read (every thread for itself: its wave's)
+  const int te = NG == 1 ? t1 : (int)min((int64_t)t1, (p.n + STEPS - 1) / STEPS);
+  if (te > t0) load(t0);
+  for (int tile = t0; tile < te; ++tile) {
     Half rv[K];
     float in[K][V], A[V], H[V], st[V];
 #pragma unroll
@@ -438,7 +440,7 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
         A[j] = fmaf(-i, A[j], A[j]);
       }
     }
-    if (tile + 1 < t1) load(tile + 1);
+    if (tile + 1 < te) load(tile + 1);
     if (a.states && p.grp == 0)
       store_n<V>(a.states + (p.b * a.tiles + tile) * a.D + p.c0, s, p.nv);
     tile_scan<LC, NG, V>(A, H, s, st, lds[tile & 1]);
@@ -458,6 +460,13 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
     };
     if (NG > 1 && (int64_t)(tile + 1) * STEPS <= p.n) replay(Yes());
     else replay(No());
+  }
+  for (int tile = max(te, t0); tile < t1; ++tile) {
+    const int64_t t = wave_step<LC, NG, K>(tile);
+    const float zero[V] = {};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (t + rh_.ls + k < a.T) store8<E, PART>(rh_.at(t, k), zero, p.nv);
   }
   if (p.grp == 0 && t1 == a.tiles) store_n<V>(a.last + ch, s, p.nv);
 }
@@ -486,7 +495,9 @@ __global__ void __launch_bounds__(LC * NG) rec_sum_kernel(const RecArgs a) {
     A[j] = 1.f;
     H[j] = 0.f;
   }
-  for (int q = 0; q < a.tps; ++q) {
+  // (a segment wholly behind the end changes nothing)
+  const int rounds = (int64_t)p.seg * a.tps * STEPS < p.n ? a.tps : 0;
+  for (int q = 0; q < rounds; ++q) {
     Half rx[K], rg[K];
     const int64_t t = first + (FWD ? q * K : run - 1 - q * K);
 #pragma unroll
@@ -572,8 +583,20 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
     if (NG > 1 && (int64_t)(tile + 1) * STEPS <= p.n) load_as(tile, Yes());
     else load_as(tile, No());
   };
-  if (t1 > t0) load(t1 - 1);
-  for (int tile = t1 - 1; tile >= t0; --tile) {
+  // tiles wholly behind the sequence's end: nothing to read
+  const int te = NG == 1 ? t1 : (int)min((int64_t)t1, (p.n + STEPS - 1) / STEPS);
+  for (int tile = max(te, t0); tile < t1; ++tile) {
+    const int64_t t = wave_step<LC, NG, K>(tile);
+    const float zero[V] = {};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (t + rdv_.ls + k < a.T) {
+        store8<E, PART>(rdv_.at(t, k), zero, p.nv);
+        store8<E, PART>(rdg_.at(t, k), zero, p.nv);
+      }
+  }
+  if (te > t0) load(te - 1);
+  for (int tile = te - 1; tile >= t0; --tile) {
     Half rd[K];
     float in[K][V], e[K][V], A[V], H[V], G[V], s[V], st[V], rt[V];
 #pragma unroll

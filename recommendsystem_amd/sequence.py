@@ -66,8 +66,8 @@ def _check_norm(x, gamma, beta, epsilon):
             raise TypeError(f"layer_norm: {name} must be float32, got {p.dtype}")
         if p.shape != (D,):
             raise ValueError(f"layer_norm: {name} {tuple(p.shape)} does not fit a last dimension of {D}")
-    if not epsilon > 0:
-        raise ValueError(f"layer_norm: epsilon must be positive, got {epsilon}")
+    if not 1.2e-38 < epsilon < 3.4e38:
+        raise ValueError(f"layer_norm: epsilon must be a positive float32 number, got {epsilon}")
     return code
 
 
@@ -81,8 +81,9 @@ def _norm_forward(x, gamma, beta, epsilon, code, stats, save_8bit, stream):
     if save_8bit:
         codes = x.new_empty(x.shape, dtype=torch.int8)
         scales = gamma.new_empty(scale_shape(x.shape))
-    call("rs_layernorm_fwd", stream, code, x2.data_ptr(), x2.stride(0), R, D,
-         gamma.contiguous().data_ptr(), beta.contiguous().data_ptr(), epsilon, y.data_ptr(), D,
+    gamma, beta = gamma.contiguous(), beta.contiguous()  # (copies live until after the launch)
+    call("rs_layernorm_fwd", stream, code, x2.data_ptr(), x2.stride(0), R, D, gamma.data_ptr(),
+         beta.data_ptr(), epsilon, y.data_ptr(), D,
          ptr(mean), mean.data_ptr() + 4 * R if stats else None, ptr(codes), ptr(scales))
     return y, mean, codes, scales
 
@@ -97,9 +98,10 @@ def _norm_backward(dy, x, codes, scales, gamma, mean, code, dparams, accumulate,
         dparams = gamma.new_empty((2, D))
     ws_n = _norm_workspace(R, D)
     ws = gamma.new_empty(ws_n)
+    gamma = gamma.contiguous()
     call("rs_layernorm_bwd", stream, code, dy2.data_ptr(), dy2.stride(0), ptr(x2),
          x2.stride(0) if x2 is not None else 0, ptr(codes), ptr(scales), R, D,
-         gamma.contiguous().data_ptr(), mean.data_ptr(), mean.data_ptr() + 4 * R, dx.data_ptr(), D,
+         gamma.data_ptr(), mean.data_ptr(), mean.data_ptr() + 4 * R, dx.data_ptr(), D,
          dparams.data_ptr(), dparams.data_ptr() + 4 * D, accumulate, ws.data_ptr(), ws_n)
     return dx, dparams
 
@@ -120,6 +122,7 @@ class _LayerNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, codes, scales, gamma, beta, mean = ctx.saved_tensors
         code, in_place, index = ctx.args
+        in_place = in_place and ctx.needs_input_grad[1] and ctx.needs_input_grad[2]
         block = grads_contiguous((gamma, beta)) if in_place else None
         dx, dparams = run_on(index, _norm_backward, dy, x, codes, scales, gamma, mean, code, block,
                              block is not None)
@@ -418,13 +421,13 @@ class SequenceEncoder(nn.Module):
         self.recurrences = nn.ModuleList(
             GatedRecurrence(units, forget_bias, seed + 2 * k, save_8bit, device) for k in range(depth))
         self._out = [dict(seed=seed + 2 * k + 1, device=device, save_8bit=save_8bit) for k in range(depth)]
-        self.outputs = nn.ModuleList()
         self.final = LayerNormalization(epsilon, save_8bit, device)
         self.built = False
         self.name = name
 
     def build(self, input_shape, device=None):
         E = int(input_shape[-1])
+        self.outputs = nn.ModuleList()
         for k in range(self.depth):
             self.norms[k].build((E,), device)
             self.recurrences[k].build((E,), device)

@@ -217,6 +217,25 @@ def test_layer_norm_strides_ranks_and_empty():
     assert dx.shape == x.shape and not dg.any() and not db.any()
 
 
+def test_layer_norm_parameters_of_any_stride_and_frozen():
+    """gamma and beta as columns of one matrix; a frozen beta's gradient buffer is left alone."""
+    p = rnd(40, 2)
+    x, dy = rnd(6, 40), rnd(6, 40)
+    gamma, beta = p[:, 0].requires_grad_(), p[:, 1].requires_grad_()
+    y = layer_norm(x, gamma, beta)
+    got = (y, *torch.autograd.grad(y, (gamma, beta), dy))
+    want = ref_norm(x, gamma, beta, 1e-5, dy)
+    for a, (w, b) in zip(got, (want[0], want[2], want[3])):
+        near(a, w, b, "strided parameters")
+    ln = LayerNormalization()
+    ln.build((40,))
+    ln.beta.requires_grad_(False)
+    ln.beta.grad.fill_(7.0)
+    ln(x).backward(dy)
+    near(ln.gamma.grad, *ref_norm(x, ln.gamma, ln.beta, 1e-5, dy)[2], "dgamma")
+    assert bool((ln.beta.grad == 7.0).all())
+
+
 def test_layer_norm_differences():
     """The gradient against central differences of the 64-bit loss of the fp32 output: with a step
     h = 2^-5 the quotient is off by h^2/6 of a third derivative (of order 1 a unit direction) and by
