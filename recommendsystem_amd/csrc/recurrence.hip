@@ -369,6 +369,38 @@ struct ScanLds {
   static constexpr int FLOATS = NG == 1 ? 1 : NG / (64 / LC) * NT * LC * V;
 };
 
+// s behind the segments from .. to - 1 (against time for !UP), whose (A, H) are in the workspace:
+// every group joins a run of them, the groups are joined as those of a tile.  lds: the buffer that
+// the first tile does not use.
+template <class E, int LC, int NG, bool UP>
+__device__ __forceinline__ void segment_fold(const RecArgs& a, const Place<E, LC, NG>& p, int from,
+                                             int to, int64_t ch, float* s, float* lds) {
+  constexpr int V = VC<E>::V;
+  const int per = (to - from + NG - 1) / NG;
+  const int lo = min(to, from + p.grp * per), hi = min(to, lo + per);
+  float A[V], H[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    A[j] = 1.f;
+    H[j] = 0.f;
+  }
+  for (int k = 0; k < hi - lo; ++k) {
+    float A2[V], H2[V];
+    const float* w = a.ws + (int64_t)(UP ? lo + k : hi - 1 - k) * 2 * a.B * a.D + ch;
+    load_n<V>(A2, w, p.nv);
+    load_n<V>(H2, w + a.B * a.D, p.nv);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      join(A[j], H[j], A2[j], H2[j]);
+      A[j] = A2[j];
+      H[j] = H2[j];
+    }
+  }
+  tile_total<LC, NG, V, UP>(A, H, lds);
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[j] = pass(s[j], A[j], H[j]);
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------------------------------------
@@ -391,14 +423,8 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = 0.f;
   if (a.h0) load_n<V>(s, a.h0 + ch, p.nv);
-  for (int k = 0; k < p.seg; ++k) {
-    float A[V], H[V];
-    const float* w = a.ws + (int64_t)k * 2 * a.B * a.D + ch;
-    load_n<V>(A, w, p.nv);
-    load_n<V>(H, w + a.B * a.D, p.nv);
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = pass(s[j], A[j], H[j]);
-  }
+  if (NG > 1 && p.seg > 0)
+    segment_fold<E, LC, NG, true>(a, p, 0, p.seg, ch, s, lds[(t0 & 1) ^ 1]);
 
   Half nv_[K], ng_[K];
   // (whole: every step of the tile is part of the sequence)
@@ -553,14 +579,8 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
 #pragma unroll
   for (int j = 0; j < V; ++j) r[j] = 0.f;
   if (a.dlast) load_n<V>(r, a.dlast + ch, p.nv);
-  for (int k = a.segs - 1; k > p.seg; --k) {
-    float A[V], G[V];
-    const float* w = a.ws + (int64_t)k * 2 * a.B * a.D + ch;
-    load_n<V>(A, w, p.nv);
-    load_n<V>(G, w + a.B * a.D, p.nv);
-#pragma unroll
-    for (int j = 0; j < V; ++j) r[j] = pass(r[j], A[j], G[j]);
-  }
+  if (NG > 1 && p.seg + 1 < a.segs)
+    segment_fold<E, LC, NG, false>(a, p, p.seg + 1, a.segs, ch, r, lds[t1 & 1]);
 
   Half nv_[K], ng_[K], nd_[K];
   float ns[V];
