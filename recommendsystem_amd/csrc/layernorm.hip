@@ -8,9 +8,13 @@
 // constant row is normalised to exact zeros.
 //
 // Bound by memory.  A row lives in the registers of TPR threads (1 .. 64 lanes of a wave, or 2 to 8
-// waves), NCH x 16 bytes each, so it is read once; workgroups stay and walk the rows, with gamma and beta in registers and the next row's loads in flight.  In the backward every
-// thread also keeps its columns' share of dgamma and dbeta in registers over all of its rows; one
-// partial row a workgroup then goes to the workspace and a second launch adds them in a fixed order.
+// waves), NCH x 16 bytes each, so it is read once; workgroups stay and walk the rows, with gamma and
+// beta in registers and the next row's loads in flight.  In the backward every thread also keeps its
+// columns' share of dgamma and dbeta in registers over all of its rows; one partial row a workgroup
+// then goes to the workspace and a second launch adds them in a fixed order.
+// 65536 x 1024 bf16: forward 46 us (5.8 TB/s), backward 78 + 4 us (5.2 TB/s); a large copy of torch's
+// runs at 5.4 TB/s.  Rows that start off 16 bytes cost more, each load then touching two pieces of 64
+// bytes: 40000 x 1500 bf16 forward 5.5, backward 3.5 TB/s; 4099 x 5003 fp16 3.7 and 2.9 TB/s.
 #include "elem.hpp"
 
 #define LN_MAX_D 32768

@@ -358,6 +358,26 @@ def test_gated_recurrence(B, T, D, dtype, ragged):
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
 
 
+@pytest.mark.parametrize("B,T,D", [(1, 6000, 24), (2, 5000, 1030), (3, 4100, 700)])
+def test_recurrence_segments_that_end_anywhere(B, T, D):
+    """Long ragged histories, whose time axis is cut: ends in front of, inside and behind a segment,
+    on the edge of a tile, and nowhere, with the same bits every time."""
+    v, g, h0 = rnd(B, T, D), rnd(B, T, D, mean=1.0), rnd(B, D)
+    dh, dlast = rnd(B, T, D), rnd(B, D)
+    leaves = [t.requires_grad_() for t in (v, g, h0)]
+    for ends in ((0, 1, T), (255, 256, 257), (T - 1, 1000, 1151), (2048, T // 2, 129)):
+        lengths = torch.tensor(ends[:B], device=DEV)
+        h, last = gated_recurrence(*leaves, lengths)
+        got = (h, last, *torch.autograd.grad((h, last), leaves, (dh, dlast)))
+        want = ref_rec(v.detach(), g.detach(), h0.detach(), lengths, dh, dlast)
+        for a, (w, b), what in zip(got, want, ("h", "last", "dv", "dg", "dh0")):
+            near(a, w, b, f"{what} with ends {ends[:B]}")
+        for _ in range(3):
+            h, last = gated_recurrence(*leaves, lengths)
+            again = (h, last, *torch.autograd.grad((h, last), leaves, (dh, dlast)))
+            assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
 def test_recurrence_partial_arguments():
     """No state before, one output's gradient only, the joint form, int64 and odd lengths, strides."""
     B, T, D = 3, 70, 24
