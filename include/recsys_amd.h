@@ -863,7 +863,7 @@ int rs_ctr_metrics_result(void* stream, const double* state, int nthr, float* ou
 /* 8-bit form of x [rows, D] (contiguous codes [rows, D], scales [rows, ceil(D / 128)]): in each
  * block of 128 columns scale = max|x| / 127 in fp32 and code = x / scale to the nearest whole
  * number, ties to even.  A block with max|x| < 2^-100 reads back as zeros, one that holds an
- * infinity or NaN as NaN.  rs_unpack8: y = code * scale. */
+ * infinity or NaN as NaN.  rs_unpack8: y = code * scale.  D <= 2^30. */
 int rs_pack8(void* stream, int dtype, const void* x, int64_t ld_x, int64_t rows, int D,
              int8_t* codes, float* scales);
 int rs_unpack8(void* stream, int dtype, const int8_t* codes, const float* scales, int64_t rows,

@@ -111,7 +111,7 @@ int unpack8(hipStream_t s, const int8_t* codes, const float* scales, int64_t row
 
 RS_API int rs_pack8(void* stream, int dtype, const void* x, int64_t ld_x, int64_t rows, int D,
                     int8_t* codes, float* scales) {
-  if (rows < 0 || D <= 0 || dtype < RS_F32 || dtype > RS_F16) return RS_ERR_ARG;
+  if (rows < 0 || D <= 0 || D > 1 << 30 || dtype < RS_F32 || dtype > RS_F16) return RS_ERR_ARG;
   if (rows == 0) return RS_OK;
   if (!x || !codes || !scales || ld_x < 0) return RS_ERR_ARG;
   return RS_DISPATCH_ELEM(dtype, pack8, rs_stream(stream), x, ld_x, rows, D, codes, scales);
@@ -119,7 +119,7 @@ RS_API int rs_pack8(void* stream, int dtype, const void* x, int64_t ld_x, int64_
 
 RS_API int rs_unpack8(void* stream, int dtype, const int8_t* codes, const float* scales,
                       int64_t rows, int D, void* y, int64_t ld_y) {
-  if (rows < 0 || D <= 0 || dtype < RS_F32 || dtype > RS_F16) return RS_ERR_ARG;
+  if (rows < 0 || D <= 0 || D > 1 << 30 || dtype < RS_F32 || dtype > RS_F16) return RS_ERR_ARG;
   if (rows == 0) return RS_OK;
   if (!codes || !scales || !y || ld_y < D) return RS_ERR_ARG;
   return RS_DISPATCH_ELEM(dtype, unpack8, rs_stream(stream), codes, scales, rows, D, y, ld_y);

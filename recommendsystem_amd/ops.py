@@ -33,7 +33,7 @@ from . import _lib, packing, sequence
 from ._lib import call, ptr, stream_handle
 
 _U64 = 0xFFFFFFFFFFFFFFFF
-_USE = {"on": False}
+_USE = _lib.CUSTOM_OPS
 
 
 def use_custom_ops(on: bool = True) -> None:

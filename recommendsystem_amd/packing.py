@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import call, device_index, ptr, run_on
+from ._lib import call, device_index, empty, run_on
 
 BLOCK = 128
 ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -37,7 +37,7 @@ def rows_of(t: torch.Tensor) -> torch.Tensor:
 def _width(x: torch.Tensor, what: str) -> int:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what} needs a last dimension of at least 1, got shape {tuple(x.shape)}")
-    if x.shape[-1] >= 2 ** 31:
+    if x.shape[-1] > 2 ** 30:
         raise ValueError(f"{what}: a last dimension of {x.shape[-1]} is not supported")
     return x.shape[-1]
 
@@ -56,9 +56,9 @@ def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _pack(x, D, code, stream):
     x2 = rows_of(x)
-    codes = x.new_empty(x.shape, dtype=torch.int8)
-    scales = x.new_empty(scale_shape(x.shape), dtype=torch.float32)
-    call("rs_pack8", stream, code, ptr(x2), x2.stride(0), x2.shape[0], D, ptr(codes), ptr(scales))
+    codes, scales = empty(x.shape, torch.int8), empty(scale_shape(x.shape))
+    call("rs_pack8", stream, code, x2.data_ptr(), x2.stride(0), x2.shape[0], D, codes.data_ptr(),
+         scales.data_ptr())
     return codes, scales
 
 
@@ -77,7 +77,7 @@ def unpack8(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.float32) -> t
 
 def _unpack(codes, scales, D, dtype, stream):
     codes, scales = codes.contiguous(), scales.contiguous()
-    y = scales.new_empty(codes.shape, dtype=dtype)
-    call("rs_unpack8", stream, ELEMENT_TYPES[dtype], ptr(codes), ptr(scales), codes.numel() // D, D,
-         ptr(y), D)
+    y = empty(codes.shape, dtype)
+    call("rs_unpack8", stream, ELEMENT_TYPES[dtype], codes.data_ptr(), scales.data_ptr(),
+         codes.numel() // D, D, y.data_ptr(), D)
     return y

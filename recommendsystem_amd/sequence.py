@@ -25,7 +25,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, device_index, ptr, run_on
+from ._lib import call, device_index, empty, ptr, run_on
 from .layers import Dense
 from .packing import element_code, pack8, rows_of, scale_shape, unpack8  # noqa: F401
 from .params import FlatBlock, grads_contiguous
@@ -74,13 +74,12 @@ def _check_norm(x, gamma, beta, epsilon):
 def _norm_forward(x, gamma, beta, epsilon, code, stats, save_8bit, stream):
     x2 = rows_of(x)
     R, D = x2.shape
-    y = x.new_empty(x.shape)
+    y = empty(x.shape, x.dtype)
     mean = codes = scales = None  # mean: [means | 1 / standard deviations]
     if stats:
-        mean = gamma.new_empty((2, R))
+        mean = empty((2, R))
     if save_8bit:
-        codes = x.new_empty(x.shape, dtype=torch.int8)
-        scales = gamma.new_empty(scale_shape(x.shape))
+        codes, scales = empty(x.shape, torch.int8), empty(scale_shape(x.shape))
     gamma, beta = gamma.contiguous(), beta.contiguous()  # (copies live until after the launch)
     call("rs_layernorm_fwd", stream, code, x2.data_ptr(), x2.stride(0), R, D, gamma.data_ptr(),
          beta.data_ptr(), epsilon, y.data_ptr(), D,
@@ -93,11 +92,11 @@ def _norm_backward(dy, x, codes, scales, gamma, mean, code, dparams, accumulate,
     dy2 = rows_of(dy)
     R, D = dy2.shape
     x2 = rows_of(x) if x is not None else None
-    dx = dy.new_empty(dy.shape)
+    dx = empty(dy.shape, dy.dtype)
     if dparams is None:
-        dparams = gamma.new_empty((2, D))
+        dparams = empty((2, D))
     ws_n = _norm_workspace(R, D)
-    ws = gamma.new_empty(ws_n)
+    ws = empty((ws_n,))
     gamma = gamma.contiguous()
     call("rs_layernorm_bwd", stream, code, dy2.data_ptr(), dy2.stride(0), ptr(x2),
          x2.stride(0) if x2 is not None else 0, ptr(codes), ptr(scales), R, D,
@@ -134,8 +133,7 @@ def _norm(x, gamma, beta, epsilon, save_8bit, in_place):
     code = _check_norm(x, gamma, beta, epsilon)
     index = device_index(x, gamma, beta)
     if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
-        from . import ops
-        if ops.custom_ops_enabled() and not save_8bit:
+        if _lib.CUSTOM_OPS["on"] and not save_8bit:
             return torch.ops.ctr.layer_norm(x, gamma, beta, epsilon)[0]
         return _LayerNormFn.apply(x, gamma, beta, epsilon, code, save_8bit, in_place, index)
     return run_on(index, _norm_forward, x, gamma, beta, epsilon, code, False, False)[0]
@@ -243,10 +241,10 @@ def _rec_forward(v, g, h0, lengths, code, keep, stream):
     v, v_sb, v_st = _strided(v)
     g, g_sb, g_st = _strided(g)
     n_states, n_ws = _rec_sizes(code, B, T, D)
-    h = v.new_empty((B, T, D))
-    last = v.new_empty((B, D), dtype=torch.float32)
-    states = last.new_empty(n_states) if keep and n_states else None
-    ws = last.new_empty(n_ws) if n_ws else None
+    h = empty((B, T, D), v.dtype)
+    last = empty((B, D))
+    states = empty((n_states,)) if keep and n_states else None
+    ws = empty((n_ws,)) if n_ws else None
     call("rs_gated_rec_fwd", stream, code, v.data_ptr(), v_sb, v_st, g.data_ptr(), g_sb, g_st, B, T, D,
          ptr(lengths), ptr(h0), h.data_ptr(), last.data_ptr(), ptr(states), ptr(ws), n_ws)
     return h, last, states
@@ -255,8 +253,8 @@ def _rec_forward(v, g, h0, lengths, code, keep, stream):
 def _rec_backward(v, g, h0, lengths, states, dh, dlast, code, want_h0, stream):
     """(dv, dg, dh0); with g None dv is the gradient of the joint rows and dg None."""
     joint = g is None
-    dvg = v.new_empty(v.shape)
-    dv, dg = _halves(dvg, None if joint else v.new_empty(v.shape))
+    dvg = empty(v.shape, v.dtype)
+    dv, dg = _halves(dvg, None if joint else empty(v.shape, v.dtype))
     v, g = _halves(v, g)
     B, T, D = v.shape
     v, v_sb, v_st = _strided(v)
@@ -267,9 +265,9 @@ def _rec_backward(v, g, h0, lengths, states, dh, dlast, code, want_h0, stream):
         dh, dh_sb, dh_st = _strided(dh)
     if dlast is not None:
         dlast = dlast.contiguous()
-    dh0 = v.new_empty((B, D), dtype=torch.float32) if want_h0 else None
+    dh0 = empty((B, D)) if want_h0 else None
     n_ws = _rec_sizes(code, B, T, D)[1]
-    ws = v.new_empty(n_ws, dtype=torch.float32) if n_ws else None
+    ws = empty((n_ws,)) if n_ws else None
     call("rs_gated_rec_bwd", stream, code, v.data_ptr(), v_sb, v_st, g.data_ptr(), g_sb, g_st, B, T, D,
          ptr(lengths), ptr(h0), ptr(states), ptr(dh), dh_sb, dh_st, ptr(dlast), dv.data_ptr(), d_sb, d_st,
          dg.data_ptr(), d_sb, d_st, ptr(dh0), ptr(ws), n_ws)
@@ -325,8 +323,7 @@ def gated_recurrence(v, g=None, h0=None, lengths=None):
     if h0 is not None:
         h0 = h0.contiguous()
     if torch.is_grad_enabled() and _any_grad(v, g, h0):
-        from . import ops
-        if ops.custom_ops_enabled():
+        if _lib.CUSTOM_OPS["on"]:
             return tuple(torch.ops.ctr.gated_recurrence(v, g, h0, lengths)[:2])
         return _RecurrenceFn.apply(v, g, h0, lengths, code, index)
     return run_on(index, _rec_forward, v, g, h0, lengths, code, False)[:2]
@@ -355,9 +352,9 @@ def _rec_step(v, g, state, out, B, D, code, stream):
         v, g = (t if t.stride(1) == 1 else t.contiguous() for t in (v, g))
     if state is not None:
         state = state.contiguous()
-    h = v.new_empty((B, D))
+    h = empty((B, D), v.dtype)
     if out is None:
-        out = v.new_empty((B, D), dtype=torch.float32)
+        out = empty((B, D))
     call("rs_gated_rec_step", stream, code, v.data_ptr(), v.stride(0), g.data_ptr(), g.stride(0), B, D,
          ptr(state), h.data_ptr(), out.data_ptr())
     return h, out

@@ -581,6 +581,37 @@ def test_offsets_past_32_bits():
 # ============================================================================================
 # together: the encoder, Dense with an 8-bit input, the custom operators
 # ============================================================================================
+def test_second_derivatives_are_refused():
+    """create_graph gives the same first derivatives; asking for a second raises."""
+    x, g = rnd(2, 9, 12).requires_grad_(), rnd(2, 9, 12).requires_grad_()
+    gamma, beta = rnd(12).requires_grad_(), rnd(12).requires_grad_()
+    for run in (lambda: layer_norm(x, gamma, beta), lambda: layer_norm(x, gamma, beta, 1e-5, True),
+                lambda: gated_recurrence(x, g)[0]):
+        want, = torch.autograd.grad(run().square().sum(), x)
+        got, = torch.autograd.grad(run().square().sum(), x, create_graph=True)
+        assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            got.sum().backward()
+
+
+def test_inference_mode_and_two_streams():
+    """Under inference mode, and two calls in flight at once."""
+    x, g = rnd(3, 5000, 64), rnd(3, 5000, 64)
+    gamma, beta = rnd(64), rnd(64)
+    want = gated_recurrence(layer_norm(x, gamma, beta), g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    with torch.inference_mode():
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                outs.append([gated_recurrence(layer_norm(x, gamma, beta), g) for _ in range(4)])
+        torch.cuda.synchronize()
+    for run in outs:
+        for h, last in run:
+            assert torch.equal(h, want[0]) and torch.equal(last, want[1])
+
+
 def test_dense_save_8bit():
     a, b = Dense(20, "relu", seed=3), Dense(20, "relu", seed=3, save_8bit=True)
     x = rnd(65, 300)

@@ -80,6 +80,7 @@ def test_entry_points_reject():
     assert lib.rs_pack8(None, 3, p, 4, 1, 4, p, p) == ARG           # type
     assert lib.rs_pack8(None, 0, None, 4, 1, 4, p, p) == ARG
     assert lib.rs_pack8(None, 0, p, 4, 1, 0, p, p) == ARG
+    assert lib.rs_pack8(None, 0, p, 4, 1, (1 << 30) + 1, p, p) == ARG
     assert lib.rs_pack8(None, 0, None, 4, 0, 4, None, None) == 0    # no rows
     assert lib.rs_unpack8(None, 0, p, p, 1, 4, p, 3) == ARG         # ld_y < D
     assert lib.rs_layernorm_fwd(None, 0, p, 4, 1, 32769, p, p, 1e-5, p, 32769, None, None, None, None) == UNS
