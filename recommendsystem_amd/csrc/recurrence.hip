@@ -24,9 +24,13 @@
 //
 // Bound by memory; 8 bytes a lane (16 lanes to a line of 128 bytes) rather than 16 because the join
 // costs a fixed number of operations a channel and thread: twice the steps a thread, half the joins.
-// 8 x 4096 x 2048 bf16 (256 workgroups): forward 87 us (4.6 TB/s), backward 165 us (4.1 TB/s), and no
-// faster without any arithmetic (83 and 147 us): rows are read in pieces of 128 bytes.  In pieces of
-// 256 bytes, 8 x 4096 x 4096 bf16: 149 us (5.4 TB/s) and 285 us (4.7 TB/s).
+// Tiles that are wholly part of the sequence go through a loop of their own with nothing conditional
+// around its loads and stores: only then does the compiler know how many are in flight, and waits for
+// the next tile's loads without waiting for this tile's stores (8 x 4096 x 2048 bf16, backward: 146 us,
+// 175 us where both were waited for; 10 x 4096 x 2048: 214 against 271; 37 x 1021 x 520 fp32: 109 against 126).
+// 8 x 4096 x 2048 bf16 (256 workgroups, pieces of 128 bytes): forward 85 to 94 us (4.5 TB/s), backward
+// 146 us (4.6 TB/s).  8 x 4096 x 4096 in pieces of 256 bytes: 155 us (5.2 TB/s) and 268 us (5.0 TB/s),
+// as fast as a copy of that size.
 #include "elem.hpp"
 
 namespace {
@@ -69,47 +73,53 @@ template <class E>
 struct VC { static constexpr int V = 8 / (int)sizeof(typename E::T); };
 struct Half { uint32_t w[2]; };
 
-// The row's channels at p (8 bytes), or `fill` where the step is not part of the sequence (in =
-// false; p then points at some row that is).  PART (D is no multiple of V): a lane with fewer than
-// V channels left picks its nv elements one by one (none for nv <= 0); without it every lane reads 8
-// bytes (lanes without channels read those of channel 0: Place).
+// The row's channels at p (8 bytes).  PART (D is no multiple of V): a lane with fewer than V channels
+// left picks its nv elements one by one (none for nv <= 0).  Without it every lane has V channels
+// (Place), and nothing is conditional: a load or store behind a branch would leave the number of
+// memory operations in flight unknown, and the next tile's loads could then only be waited for
+// together with all of this tile's stores.  For the same reason steps that are not part of the
+// sequence are loaded from some row that is, and masked where they are used.
 template <class E, bool PART>
-__device__ __forceinline__ void load8(Half& r, const typename E::T* p, int nv, bool in, uint32_t fill) {
+__device__ __forceinline__ void load8(Half& r, const typename E::T* p, int nv) {
   constexpr int V = VC<E>::V, S = 8 / V;
   if (!PART || nv >= V) {
     const RsVec<8, S> x = *reinterpret_cast<const RsVec<8, S>*>(p);
-    r.w[0] = in ? x.w[0] : fill;
-    r.w[1] = in ? x.w[1] : fill;
+    r.w[0] = x.w[0];
+    r.w[1] = x.w[1];
   } else {
-    r.w[0] = r.w[1] = fill;
-    if (in && nv > 0) {
+    r.w[0] = r.w[1] = 0;
+    if (nv > 0) {
       if (S == 4) r.w[0] = reinterpret_cast<const uint32_t*>(p)[0];
       else {
         const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-        r.w[0] = (fill & 0xFFFF0000u) | h[0];
-        if (nv > 1) r.w[0] = (r.w[0] & 0xFFFFu) | ((uint32_t)h[1] << 16);
-        if (nv > 2) r.w[1] = (fill & 0xFFFF0000u) | h[2];
+        r.w[0] = h[0];
+        if (nv > 1) r.w[0] |= (uint32_t)h[1] << 16;
+        if (nv > 2) r.w[1] = h[2];
       }
     }
   }
 }
+__device__ __forceinline__ void mask8(Half& r, bool in, uint32_t fill) {
+  r.w[0] = in ? r.w[0] : fill;
+  r.w[1] = in ? r.w[1] : fill;
+}
 template <class E, bool PART>
 __device__ __forceinline__ void store8(typename E::T* p, const float* x, int nv) {
   constexpr int V = VC<E>::V, S = 8 / V;
-  if (PART ? nv >= V : nv > 0) {
+  if (!PART || nv >= V) {
     RsVec<8, S> y;
     E::template pack<2>(x, y.w);
     *reinterpret_cast<RsVec<8, S>*>(p) = y;
-  } else if (PART) {
+  } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
       if (j < nv) p[j] = E::store(x[j]);
   }
 }
 // V floats (states, gradients of them)
-template <int V>
+template <int V, bool PART>
 __device__ __forceinline__ void load_n(float* x, const float* p, int nv) {
-  if (nv >= V) {
+  if (!PART || nv >= V) {
     const RsVec<4 * V, 4> r = *reinterpret_cast<const RsVec<4 * V, 4>*>(p);
 #pragma unroll
     for (int j = 0; j < V; ++j) x[j] = __uint_as_float(r.w[j]);
@@ -118,9 +128,9 @@ __device__ __forceinline__ void load_n(float* x, const float* p, int nv) {
     for (int j = 0; j < V; ++j) x[j] = j < nv ? p[j] : 0.f;
   }
 }
-template <int V>
+template <int V, bool PART>
 __device__ __forceinline__ void store_n(float* p, const float* x, int nv) {
-  if (nv >= V) {
+  if (!PART || nv >= V) {
     RsVec<4 * V, 4> r;
 #pragma unroll
     for (int j = 0; j < V; ++j) r.w[j] = __float_as_uint(x[j]);
@@ -150,10 +160,12 @@ __device__ __forceinline__ unsigned xcd_run(unsigned id, unsigned n) {
 }
 
 // Which (b, channels, segment) a thread works on.
-template <class E, int LC, int NG>
+// Lanes beyond the width (PART excepted) or the batch do the last ones' work once more, and write the
+// same values to the same places.
+template <class E, int LC, int NG, bool PART>
 struct Place {
   int64_t b;
-  int c0, nv;  // first channel, channels in range (<= 0: none)
+  int c0, nv;  // first channel, channels in range (PART: down to 0 or below)
   int cl;      // the channel to load from: c0, or 0 where there is none in range
   int seg, grp;
   int64_t n;   // steps of this sequence
@@ -161,11 +173,10 @@ struct Place {
     const int tid = (int)threadIdx.x;
     if (NG == 1) {  // every thread for itself: (b, 8 bytes of channels) in one flat range
       const int nch = (a.D + VC<E>::V - 1) / VC<E>::V;
-      const int64_t id = (int64_t)blockIdx.x * LC + tid;
+      int64_t id = (int64_t)blockIdx.x * LC + tid;
+      if (id >= a.B * nch) id = a.B * nch - 1;
       b = id / nch;
       c0 = (int)(id % nch) * VC<E>::V;
-      nv = b < a.B ? a.D - c0 : 0;
-      if (b >= a.B) b = a.B - 1;
       seg = 0;
       grp = 0;
     } else {
@@ -175,9 +186,10 @@ struct Place {
       id -= seg * per;
       b = id / a.nct;
       c0 = ((int)(id % a.nct) * LC + tid % LC) * VC<E>::V;
-      nv = a.D - c0;
       grp = tid / LC;
     }
+    if (!PART && c0 > a.D - VC<E>::V) c0 = a.D - VC<E>::V;
+    nv = a.D - c0;
     cl = nv > 0 ? c0 : 0;
     n = a.T;
     if (a.lengths) {
@@ -267,8 +279,8 @@ __device__ __forceinline__ void tile_scan(float* A, float* H, float* s, float* i
   }
   wave_scan<LC, NG, V, true>(A, H);
   if (wave_edge<LC, NG, V, true>()) {
-    store_n<V>(wave_part<LC, NG, V, 2>(lds, 0), A, V);
-    store_n<V>(wave_part<LC, NG, V, 2>(lds, 1), H, V);
+    store_n<V, false>(wave_part<LC, NG, V, 2>(lds, 0), A, V);
+    store_n<V, false>(wave_part<LC, NG, V, 2>(lds, 1), H, V);
   }
   lds_barrier();
   tile_fold<LC, NG, V, true, 2>(lds, 1, s, in);
@@ -295,10 +307,10 @@ __device__ __forceinline__ void tile_scan_both(float* A, float* H, float* G, flo
   wave_scan<LC, NG, V, true>(A, H);
   wave_scan<LC, NG, V, false>(A2, G);
   if (wave_edge<LC, NG, V, true>()) {
-    store_n<V>(wave_part<LC, NG, V, 3>(lds, 0), A, V);
-    store_n<V>(wave_part<LC, NG, V, 3>(lds, 1), H, V);
+    store_n<V, false>(wave_part<LC, NG, V, 3>(lds, 0), A, V);
+    store_n<V, false>(wave_part<LC, NG, V, 3>(lds, 1), H, V);
   }
-  if (wave_edge<LC, NG, V, false>()) store_n<V>(wave_part<LC, NG, V, 3>(lds, 2), G, V);
+  if (wave_edge<LC, NG, V, false>()) store_n<V, false>(wave_part<LC, NG, V, 3>(lds, 2), G, V);
   lds_barrier();
   tile_fold<LC, NG, V, true, 3>(lds, 1, s, in_s);
   tile_fold<LC, NG, V, false, 3>(lds, 2, r, in_r);
@@ -312,8 +324,8 @@ __device__ __forceinline__ void tile_total(float* A, float* H, float* lds) {
   constexpr int W = NG / (64 / LC);
   wave_scan<LC, NG, V, UP>(A, H);
   if (wave_edge<LC, NG, V, UP>()) {
-    store_n<V>(wave_part<LC, NG, V, 2>(lds, 0), A, V);
-    store_n<V>(wave_part<LC, NG, V, 2>(lds, 1), H, V);
+    store_n<V, false>(wave_part<LC, NG, V, 2>(lds, 0), A, V);
+    store_n<V, false>(wave_part<LC, NG, V, 2>(lds, 1), H, V);
   }
   lds_barrier();
 #pragma unroll
@@ -377,9 +389,9 @@ struct ScanLds {
 // s behind the segments from .. to - 1 (against time for !UP), whose (A, H) are in the workspace:
 // every group joins a run of them, the groups are joined as those of a tile.  lds: the buffer that
 // the first tile does not use.
-template <class E, int LC, int NG, bool UP>
-__device__ __forceinline__ void segment_fold(const RecArgs& a, const Place<E, LC, NG>& p, int from,
-                                             int to, int64_t ch, float* s, float* lds) {
+template <class E, int LC, int NG, bool PART, bool UP>
+__device__ __forceinline__ void segment_fold(const RecArgs& a, const Place<E, LC, NG, PART>& p,
+                                             int from, int to, int64_t ch, float* s, float* lds) {
   constexpr int V = VC<E>::V;
   const int per = (to - from + NG - 1) / NG;
   const int lo = min(to, from + p.grp * per), hi = min(to, lo + per);
@@ -392,8 +404,8 @@ __device__ __forceinline__ void segment_fold(const RecArgs& a, const Place<E, LC
   for (int k = 0; k < hi - lo; ++k) {
     float A2[V], H2[V];
     const float* w = a.ws + (int64_t)(UP ? lo + k : hi - 1 - k) * 2 * a.B * a.D + ch;
-    load_n<V>(A2, w, p.nv);
-    load_n<V>(H2, w + a.B * a.D, p.nv);
+    load_n<V, PART>(A2, w, p.nv);
+    load_n<V, PART>(H2, w + a.B * a.D, p.nv);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       join(A[j], H[j], A2[j], H2[j]);
@@ -416,7 +428,7 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
   constexpr int V = VC<E>::V, STEPS = NG * K;
   typedef typename E::T X;
   __shared__ __attribute__((aligned(16))) float lds[2][ScanLds<LC, NG, V, 2>::FLOATS];
-  const Place<E, LC, NG> p(a);
+  const Place<E, LC, NG, PART> p(a);
   typedef Rows<E, LC, NG, K, const X*> In;
   const In rv_((const X*)a.v, p.b, a.v_sb, a.v_st, p.cl), rg_((const X*)a.g, p.b, a.g_sb, a.g_st, p.cl);
   const Rows<E, LC, NG, K, X*> rh_((X*)a.h, p.b, a.T * a.D, a.D, p.c0);
@@ -427,30 +439,25 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
   float s[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = 0.f;
-  if (a.h0) load_n<V>(s, a.h0 + ch, p.nv);
+  if (a.h0) load_n<V, PART>(s, a.h0 + ch, p.nv);
   if (NG > 1 && p.seg > 0)
-    segment_fold<E, LC, NG, true>(a, p, 0, p.seg, ch, s, lds[(t0 & 1) ^ 1]);
+    segment_fold<E, LC, NG, PART, true>(a, p, 0, p.seg, ch, s, lds[(t0 & 1) ^ 1]);
 
   Half nv_[K], ng_[K];
   // (whole: every step of the tile is part of the sequence)
-  auto load_as = [&](int tile, auto whole) __attribute__((always_inline)) {
+  auto load = [&](int tile, auto whole) __attribute__((always_inline)) {
+    constexpr bool W = decltype(whole)::value;
     const int64_t t = wave_step<LC, NG, K>(tile);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      constexpr bool W = decltype(whole)::value;
-      const bool in = W || t + rv_.ls + k < p.n;
-      load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, some), p.nv, in, 0u);
-      load8<E, PART>(ng_[k], W ? rg_.at(t, k) : rg_.in(t, k, some), p.nv, in, ShutGate<E>::W);
+      load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, some), p.nv);
+      load8<E, PART>(ng_[k], W ? rg_.at(t, k) : rg_.in(t, k, some), p.nv);
     }
   };
-  auto load = [&](int tile) __attribute__((always_inline)) {
-    if (NG > 1 && (int64_t)(tile + 1) * STEPS <= p.n) load_as(tile, Yes());
-    else load_as(tile, No());
-  };
-  // tiles wholly behind the sequence's end: nothing to read (every thread for itself: its wave's)
-  const int te = NG == 1 ? t1 : (int)min((int64_t)t1, (p.n + STEPS - 1) / STEPS);
-  if (te > t0) load(t0);
-  for (int tile = t0; tile < te; ++tile) {
+  // one tile; next: starts the next tile's loads, in between
+  auto run = [&](int tile, auto whole, auto next) __attribute__((always_inline)) {
+    constexpr bool W = decltype(whole)::value;
+    const int64_t t = wave_step<LC, NG, K>(tile);
     Half rv[K];
     float in[K][V], A[V], H[V], st[V];
 #pragma unroll
@@ -461,6 +468,10 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float g[V], v[V];
+      if (!W) {
+        mask8(nv_[k], t + rv_.ls + k < p.n, 0u);
+        mask8(ng_[k], t + rv_.ls + k < p.n, ShutGate<E>::W);
+      }
       rv[k] = nv_[k];
       E::template unpack<2>(ng_[k].w, g);
       E::template unpack<2>(rv[k].w, v);
@@ -471,27 +482,36 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
         A[j] = fmaf(-i, A[j], A[j]);
       }
     }
-    if (tile + 1 < te) load(tile + 1);
     if (a.states && p.grp == 0)
-      store_n<V>(a.states + (p.b * a.tiles + tile) * a.D + p.c0, s, p.nv);
+      store_n<V, PART>(a.states + (p.b * a.tiles + tile) * a.D + p.c0, s, p.nv);
+    next();
     tile_scan<LC, NG, V>(A, H, s, st, lds[tile & 1]);
-    auto replay = [&](auto whole) __attribute__((always_inline)) {
-      const int64_t t = wave_step<LC, NG, K>(tile);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float v[V], o[V];
-        E::template unpack<2>(rv[k].w, v);
+    for (int k = 0; k < K; ++k) {
+      float v[V], o[V];
+      E::template unpack<2>(rv[k].w, v);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          st[j] = fmaf(in[k][j], v[j] - st[j], st[j]);
-          o[j] = decltype(whole)::value || t + rh_.ls + k < p.n ? st[j] : 0.f;
-        }
-        if (decltype(whole)::value || t + rh_.ls + k < a.T) store8<E, PART>(rh_.at(t, k), o, p.nv);
+      for (int j = 0; j < V; ++j) {
+        st[j] = fmaf(in[k][j], v[j] - st[j], st[j]);
+        o[j] = W || t + rh_.ls + k < p.n ? st[j] : 0.f;
       }
-    };
-    if (NG > 1 && (int64_t)(tile + 1) * STEPS <= p.n) replay(Yes());
-    else replay(No());
+      if (W || t + rh_.ls + k < a.T) store8<E, PART>(rh_.at(t, k), o, p.nv);
+    }
+  };
+  // whole tiles up to tw, then those with the sequence's end inside, up to te, then nothing to read
+  const int tw = NG == 1 ? t0 : max(t0, (int)min((int64_t)t1, p.n / STEPS));
+  const int te = NG == 1 ? t1 : (int)min((int64_t)t1, (p.n + STEPS - 1) / STEPS);
+  if (tw > t0 + 1) {
+    // (the first by itself: the loop then starts with as many stores in flight as it goes on with)
+    load(t0, Yes());
+    run(t0, Yes(), [&]() { load(t0 + 1, Yes()); });
+    for (int tile = t0 + 1; tile + 1 < tw; ++tile) run(tile, Yes(), [&]() { load(tile + 1, Yes()); });
+  } else if (tw > t0) {
+    load(t0, Yes());
   }
+  if (tw > t0) run(tw - 1, Yes(), [&]() { if (te > tw) load(tw, No()); });
+  else if (te > t0) load(t0, No());
+  for (int tile = tw; tile < te; ++tile) run(tile, No(), [&]() { if (tile + 1 < te) load(tile + 1, No()); });
   for (int tile = max(te, t0); tile < t1; ++tile) {
     const int64_t t = wave_step<LC, NG, K>(tile);
     const float zero[V] = {};
@@ -499,7 +519,7 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
     for (int k = 0; k < K; ++k)
       if (t + rh_.ls + k < a.T) store8<E, PART>(rh_.at(t, k), zero, p.nv);
   }
-  if (p.grp == 0 && t1 == a.tiles) store_n<V>(a.last + ch, s, p.nv);
+  if (p.grp == 0 && t1 == a.tiles) store_n<V, PART>(a.last + ch, s, p.nv);
 }
 
 // (A, H) of every segment but the last (backward: of every one but the first, over dh, against
@@ -509,7 +529,7 @@ __global__ void __launch_bounds__(LC * NG) rec_sum_kernel(const RecArgs a) {
   constexpr int V = VC<E>::V, STEPS = NG * K;
   typedef typename E::T X;
   __shared__ __attribute__((aligned(16))) float lds[ScanLds<LC, NG, V, 2>::FLOATS];
-  Place<E, LC, NG> p(a);
+  Place<E, LC, NG, PART> p(a);
   if (!FWD) p.seg += 1;
   // (no dh: the gates' rows are read in its place, and not used)
   const bool none = !FWD && !a.dh;
@@ -535,12 +555,15 @@ __global__ void __launch_bounds__(LC * NG) rec_sum_kernel(const RecArgs a) {
     for (int k = 0; k < K; ++k) {
       const int64_t tk = FWD ? t + k : t - k;
       const bool in = whole || tk < p.n;
-      load8<E, PART>(rx[k], in ? xp + tk * x_st : xp, p.nv, in && !none, 0u);
-      load8<E, PART>(rg[k], in ? gp + tk * a.g_st : gp, p.nv, in, ShutGate<E>::W);
+      load8<E, PART>(rx[k], in ? xp + tk * x_st : xp, p.nv);
+      load8<E, PART>(rg[k], in ? gp + tk * a.g_st : gp, p.nv);
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float g[V], x[V];
+      const bool in = whole || (FWD ? t + k : t - k) < p.n;
+      mask8(rx[k], in && !none, 0u);
+      mask8(rg[k], in, ShutGate<E>::W);
       E::template unpack<2>(rg[k].w, g);
       E::template unpack<2>(rx[k].w, x);
 #pragma unroll
@@ -555,8 +578,8 @@ __global__ void __launch_bounds__(LC * NG) rec_sum_kernel(const RecArgs a) {
   tile_total<LC, NG, V, FWD>(A, H, lds);
   if (p.grp == 0) {
     float* w = a.ws + (int64_t)p.seg * 2 * a.B * a.D + p.b * a.D + p.c0;
-    store_n<V>(w, A, p.nv);
-    store_n<V>(w + a.B * a.D, H, p.nv);
+    store_n<V, PART>(w, A, p.nv);
+    store_n<V, PART>(w + a.B * a.D, H, p.nv);
   }
 }
 
@@ -568,7 +591,7 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
   constexpr int V = VC<E>::V, STEPS = NG * K;
   typedef typename E::T X;
   __shared__ __attribute__((aligned(16))) float lds[2][ScanLds<LC, NG, V, 3>::FLOATS];
-  const Place<E, LC, NG> p(a);
+  const Place<E, LC, NG, PART> p(a);
   typedef Rows<E, LC, NG, K, const X*> In;
   typedef Rows<E, LC, NG, K, X*> Out;
   // (no dh: the gates' rows are read in its place, and not used)
@@ -583,45 +606,32 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
   float r[V];  // the gradient from behind the tile
 #pragma unroll
   for (int j = 0; j < V; ++j) r[j] = 0.f;
-  if (a.dlast) load_n<V>(r, a.dlast + ch, p.nv);
+  if (a.dlast) load_n<V, PART>(r, a.dlast + ch, p.nv);
   // tiles wholly behind the sequence's end: nothing to read
   const int te = NG == 1 ? t1 : (int)min((int64_t)t1, (p.n + STEPS - 1) / STEPS);
   if (NG > 1 && p.seg + 1 < a.segs)
-    segment_fold<E, LC, NG, false>(a, p, p.seg + 1, a.segs, ch, r, lds[te & 1]);
+    segment_fold<E, LC, NG, PART, false>(a, p, p.seg + 1, a.segs, ch, r, lds[te & 1]);
 
   Half nv_[K], ng_[K], nd_[K];
   float ns[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) ns[j] = 0.f;
-  auto load_as = [&](int tile, auto whole) __attribute__((always_inline)) {
+  auto load = [&](int tile, auto whole) __attribute__((always_inline)) {
+    constexpr bool W = decltype(whole)::value;
     const int64_t t = wave_step<LC, NG, K>(tile);
+    if (a.states) load_n<V, PART>(ns, a.states + (p.b * a.tiles + tile) * a.D + p.c0, p.nv);
+    else if (a.h0) load_n<V, PART>(ns, a.h0 + ch, p.nv);  // one tile
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      constexpr bool W = decltype(whole)::value;
-      const bool in = W || t + rv_.ls + k < p.n;
-      load8<E, PART>(ng_[k], W ? rg_.at(t, k) : rg_.in(t, k, some), p.nv, in, ShutGate<E>::W);
-      load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, some), p.nv, in, 0u);
-      load8<E, PART>(nd_[k], W ? rd_.at(t, k) : rd_.in(t, k, some), p.nv, in && !none, 0u);
+      load8<E, PART>(ng_[k], W ? rg_.at(t, k) : rg_.in(t, k, some), p.nv);
+      load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, some), p.nv);
+      load8<E, PART>(nd_[k], W ? rd_.at(t, k) : rd_.in(t, k, some), p.nv);
     }
-    if (a.states) load_n<V>(ns, a.states + (p.b * a.tiles + tile) * a.D + p.c0, p.nv);
-    else if (a.h0) load_n<V>(ns, a.h0 + ch, p.nv);  // one tile
   };
-  auto load = [&](int tile) __attribute__((always_inline)) {
-    if (NG > 1 && (int64_t)(tile + 1) * STEPS <= p.n) load_as(tile, Yes());
-    else load_as(tile, No());
-  };
-  for (int tile = max(te, t0); tile < t1; ++tile) {
+  // one tile; next: starts the loads of the tile in front, in between
+  auto run = [&](int tile, auto whole, auto next) __attribute__((always_inline)) {
+    constexpr bool W = decltype(whole)::value;
     const int64_t t = wave_step<LC, NG, K>(tile);
-    const float zero[V] = {};
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (t + rdv_.ls + k < a.T) {
-        store8<E, PART>(rdv_.at(t, k), zero, p.nv);
-        store8<E, PART>(rdg_.at(t, k), zero, p.nv);
-      }
-  }
-  if (te > t0) load(te - 1);
-  for (int tile = te - 1; tile >= t0; --tile) {
     Half rd[K];
     float in[K][V], e[K][V], A[V], H[V], G[V], s[V], st[V], rt[V];
 #pragma unroll
@@ -633,6 +643,12 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float g[V];
+      const bool in_k = W || t + rv_.ls + k < p.n;
+      if (!W) {
+        mask8(ng_[k], in_k, ShutGate<E>::W);
+        mask8(nv_[k], in_k, 0u);
+      }
+      mask8(nd_[k], in_k && !none, 0u);
       rd[k] = nd_[k];
       E::template unpack<2>(ng_[k].w, g);
       E::template unpack<2>(nv_[k].w, e[k]);
@@ -653,7 +669,7 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
         G[j] = fmaf(-in[k][j], x, x);
       }
     }
-    if (tile > t0) load(tile - 1);
+    next();
     tile_scan_both<LC, NG, V>(A, H, G, s, r, st, rt, lds[tile & 1]);
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -665,7 +681,6 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
       }
 #pragma unroll
     for (int k = K - 1; k >= 0; --k) {
-      const int64_t t = wave_step<LC, NG, K>(tile);
       float d[V], gv[V], gg[V];
       E::template unpack<2>(rd[k].w, d);
 #pragma unroll
@@ -675,13 +690,38 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
         gg[j] = gv[j] * e[k][j] * (1.0f - i);
         rt[j] = x - gv[j];
       }
-      if (t + rdv_.ls + k < a.T) {
+      if (W || t + rdv_.ls + k < a.T) {
         store8<E, PART>(rdv_.at(t, k), gv, p.nv);
         store8<E, PART>(rdg_.at(t, k), gg, p.nv);
       }
     }
+  };
+  for (int tile = max(te, t0); tile < t1; ++tile) {
+    const int64_t t = wave_step<LC, NG, K>(tile);
+    const float zero[V] = {};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (t + rdv_.ls + k < a.T) {
+        store8<E, PART>(rdv_.at(t, k), zero, p.nv);
+        store8<E, PART>(rdg_.at(t, k), zero, p.nv);
+      }
   }
-  if (p.grp == 0 && t0 == 0 && a.dh0) store_n<V>(a.dh0 + ch, r, p.nv);
+  // those with the sequence's end inside, then whole ones from tw on
+  const int tw = NG == 1 ? t0 : max(t0, (int)min((int64_t)t1, p.n / STEPS));
+  if (te > tw) {
+    load(te - 1, No());
+    for (int tile = te - 1; tile > tw; --tile) run(tile, No(), [&]() { load(tile - 1, No()); });
+    run(tw, No(), [&]() { if (tw > t0) load(tw - 1, Yes()); });
+  } else if (tw > t0) {
+    load(tw - 1, Yes());
+  }
+  if (tw > t0 + 1) {
+    // (the first by itself: the loop then starts with as many stores in flight as it goes on with)
+    run(tw - 1, Yes(), [&]() { load(tw - 2, Yes()); });
+    for (int tile = tw - 2; tile > t0; --tile) run(tile, Yes(), [&]() { load(tile - 1, Yes()); });
+  }
+  if (tw > t0) run(t0, Yes(), [&]() {});
+  if (p.grp == 0 && t0 == 0 && a.dh0) store_n<V, PART>(a.dh0 + ch, r, p.nv);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -698,17 +738,17 @@ __global__ void __launch_bounds__(256) rec_step_kernel(const RecArgs a, float* n
   const int c0 = (int)(id % nch) * V, nv = a.D - c0;
   float s[V], v[V], g[V];
   Half rv, rg;
-  load8<E, true>(rv, (const X*)a.v + b * a.v_sb + c0, nv, true, 0u);
-  load8<E, true>(rg, (const X*)a.g + b * a.g_sb + c0, nv, true, 0u);
+  load8<E, true>(rv, (const X*)a.v + b * a.v_sb + c0, nv);
+  load8<E, true>(rg, (const X*)a.g + b * a.g_sb + c0, nv);
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = 0.f;
-  if (a.h0) load_n<V>(s, a.h0 + b * a.D + c0, nv);
+  if (a.h0) load_n<V, true>(s, a.h0 + b * a.D + c0, nv);
   E::template unpack<2>(rv.w, v);
   E::template unpack<2>(rg.w, g);
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = fmaf(rec_input_gate<E>(g[j]), v[j] - s[j], s[j]);
   store8<E, true>((X*)a.h + b * a.D + c0, s, nv);
-  store_n<V>(new_state + b * a.D + c0, s, nv);
+  store_n<V, true>(new_state + b * a.D + c0, s, nv);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -726,12 +766,13 @@ namespace {
 //   WIDE  128 steps x 256 bytes, 512 threads: rows are read in longer pieces, which memory likes, but
 //         it takes twice the channels for as many workgroups
 // Forward + backward, us, bf16 (number of 128-byte tiles):        WAVE   LONG   WIDE
-//   1024 x   50 x 1024 (16384)                                     203    810    419
-//    256 x  256 x 1024 (4096)                                      225    270    269
-//     64 x 1024 x 2048 (2048)                                      486    482    446
-//     12 x 4096 x 2048 (384)                                       510    431    410
-//      8 x 4096 x 2048 (256)                                       400    268    302
-//     37 x  300 x  333 (222)                                        78     45     94
+//   1024 x   50 x 1024 (16384)                                     207    770    433
+//    256 x  256 x 1024 (4096)                                      220    253    253
+//    128 x  512 x  512 (1024)                                      111    125    112
+//     64 x 1024 x 2048 (2048)                                      479    447    426
+//     12 x 4096 x 2048 (384)                                       414    373    353
+//      8 x 4096 x 2048 (256)                                       266    248    272
+//     37 x  300 x  333 (222)                                        62     38     68
 // Up to 128 workgroups the time axis is cut so that there are at most 256, one round (65521 x 1000
 // fp16 forward: 133 us with 16 segments, 151 with 32 in two rounds); above 128 a cut would read the
 // input twice to fill less than half of the chip more.
