@@ -757,26 +757,46 @@ __global__ void __launch_bounds__(256) rec_step_kernel(const RecArgs a, float* n
 // ---------------------------------------------------------------------------------------------
 namespace {
 
-//   FLAT  tiles of 8 steps, a thread per 8 bytes of channels, nothing to join: T <= 8, or rows that
-//         fill no more than a quarter of the other kinds' tiles, and enough of them
+//   FLAT  tiles of 8 steps, a thread per 8 bytes of channels, nothing to join: T <= 8, or narrow rows
+//         and threads enough to hide that each of them waits for its own loads
+//   SLIM  rows of up to 64 bytes: tiles of 64 steps x 32 bytes of channels, one wave
+//   SLIM_LONG  the same with 1024 steps, 512 threads, for long sequences
 //   SHORT T <= 32: tiles of 32 steps x 128 bytes of channels, one wave
 //   WAVE  tiles of 64 steps x 128 bytes of channels, 128 threads, several workgroups a compute unit:
 //         short sequences, or middling ones of many workgroups, whose first loads then overlap
 //   LONG  256 steps x 128 bytes, 512 threads, one workgroup a compute unit
 //   WIDE  128 steps x 256 bytes, 512 threads: rows are read in longer pieces, which memory likes, but
-//         it takes twice the channels for as many workgroups
+//         it takes twice the channels for as many workgroups, and an odd number of 128 bytes leaves
+//         half of a tile beyond the width
 // Forward + backward, us, bf16 (number of 128-byte tiles):        WAVE   LONG   WIDE
 //   1024 x   50 x 1024 (16384)                                     207    770    433
 //    256 x  256 x 1024 (4096)                                      220    253    253
 //    128 x  512 x  512 (1024)                                      111    125    112
 //     64 x 1024 x 2048 (2048)                                      479    447    426
 //     12 x 4096 x 2048 (384)                                       414    373    353
+//     60 x 2000 x  512 (480)                                              225    207
+//     60 x 2000 x  520 (540)                                              307    345
+//    100 x 1000 x  264 (500)                                              105    149
 //      8 x 4096 x 2048 (256)                                       266    248    272
 //     37 x  300 x  333 (222)                                        62     38     68
+// narrow rows                     FLAT   SLIM   SLIM_LONG   the best of the others
+//  12000 x    16 x  8               14     39
+//   5000 x    20 x 32               20     35                 28 (SHORT)
+//  20000 x    50 x  8               46     65
+//   9000 x   100 x 16               62     58
+//  40000 x    50 x 16 fp32         241    281
+//    512 x    50 x 16                       9       28        13 (WAVE)
+//     64 x   100 x 16                      12       15        14 (WAVE)
+//    512 x   300 x 16                      24       30        37 (WAVE)
+//     32 x   300 x 16                      21       15        25 (LONG)
+//    512 x  1000 x 16                      59       43        81 (LONG)
+//    256 x  4000 x 32                     198      136       156 (LONG)
+//     16 x  4000 x 32                     186       29        27 (LONG)
+//     64 x 20000 x  8                     890       92       245 (LONG)
 // Up to 128 workgroups the time axis is cut so that there are at most 256, one round (65521 x 1000
 // fp16 forward: 133 us with 16 segments, 151 with 32 in two rounds); above 128 a cut would read the
 // input twice to fill less than half of the chip more.
-enum { REC_FLAT, REC_SHORT, REC_WAVE, REC_LONG, REC_WIDE };
+enum { REC_FLAT, REC_SHORT, REC_WAVE, REC_LONG, REC_WIDE, REC_SLIM, REC_SLIM_LONG };
 struct RecPlan {
   int kind, steps;  // steps: of a time tile
   int nct, segs, tps;
@@ -785,26 +805,28 @@ struct RecPlan {
 
 RecPlan rec_plan(int dtype, int64_t B, int64_t T, int D) {
   const int V = dtype == RS_F32 ? 2 : 4;
-  const int n16 = (D + 16 * V - 1) / (16 * V), n32 = (n16 + 1) / 2;  // channel tiles
-  const int64_t b16 = B * n16, b32 = B * n32;
-  // (a cut sequence has workgroups enough either way: wide tiles unless much of them lies beyond D)
-  const bool wide = b32 >= 160 || (b16 <= 128 && n16 >= 8);
+  const int n4 = (D + 4 * V - 1) / (4 * V), n16 = (D + 16 * V - 1) / (16 * V), n32 = (n16 + 1) / 2;
+  const int64_t b16 = B * n16, b32 = B * n32;  // channel tiles
+  // (a cut sequence has workgroups enough either way)
+  const bool wide = n16 % 2 == 0 && (b32 >= 160 || (b16 <= 128 && n16 >= 8));
+  const int64_t threads = B * ((D + V - 1) / V);  // of FLAT
+  const bool flat = n4 <= 2 && (T <= 32 ? threads >= 16384 : T <= 512 && threads >= 65536);
+  const bool slim = n4 == 1 || (n4 == 2 && T > 32);
   RecPlan p;
-  const bool narrow = 4 * D <= 16 * V && T <= 512 && B * ((D + V - 1) / V) >= 65536;
-  p.kind = T <= 8 || narrow                  ? REC_FLAT
-           : T <= 32                         ? REC_SHORT
-           : T <= 64                         ? REC_WAVE
-           : T <= 512 && b16 >= 512          ? REC_WAVE
-           : wide                            ? REC_WIDE
-                                             : REC_LONG;
-  constexpr int STEPS[] = {8, 32, 64, 256, 128};  // by kind
+  if (T <= 8 || flat) p.kind = REC_FLAT;
+  else if (slim) p.kind = T <= 128 || (T <= 512 && B * n4 >= 256) ? REC_SLIM : REC_SLIM_LONG;
+  else if (T <= 32) p.kind = REC_SHORT;
+  else if (T <= 64 || (T <= 512 && b16 >= 512)) p.kind = REC_WAVE;
+  else p.kind = wide ? REC_WIDE : REC_LONG;
+  constexpr int STEPS[] = {8, 32, 64, 256, 128, 64, 1024};  // by kind
   p.steps = STEPS[p.kind];
-  p.nct = p.kind == REC_WIDE ? n32 : n16;
+  p.nct = p.kind == REC_WIDE ? n32 : p.kind >= REC_SLIM ? n4 : n16;
   p.tiles = (T + p.steps - 1) / p.steps;
   p.segs = 1;
   p.tps = (int)p.tiles;
   const int64_t blocks = B * p.nct;
-  if ((p.kind == REC_LONG || p.kind == REC_WIDE) && blocks <= 128 && p.tiles > 1) {
+  const bool cut = p.kind == REC_LONG || p.kind == REC_WIDE || p.kind == REC_SLIM_LONG;
+  if (cut && blocks <= 128 && p.tiles > 1) {
     const int64_t want = 256 / blocks;
     p.tps = (int)((p.tiles + want - 1) / want);
     p.segs = (int)((p.tiles + p.tps - 1) / p.tps);
@@ -835,6 +857,11 @@ int rec_fwd_as(hipStream_t s, const RecPlan& p, const RecArgs& a) {
   } else if (p.kind == REC_LONG) {
     if (p.segs > 1) rec_sum_kernel<E, 16, 32, 8, true, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
     rec_fwd_kernel<E, 16, 32, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
+  } else if (p.kind == REC_SLIM) {
+    rec_fwd_kernel<E, 4, 16, 4, PART><<<per, 64, 0, s>>>(a);
+  } else if (p.kind == REC_SLIM_LONG) {
+    if (p.segs > 1) rec_sum_kernel<E, 4, 128, 8, true, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
+    rec_fwd_kernel<E, 4, 128, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
   } else {
     if (p.segs > 1) rec_sum_kernel<E, 32, 16, 8, true, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
     rec_fwd_kernel<E, 32, 16, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
@@ -855,6 +882,11 @@ int rec_bwd_as(hipStream_t s, const RecPlan& p, const RecArgs& a) {
   } else if (p.kind == REC_LONG) {
     if (p.segs > 1) rec_sum_kernel<E, 16, 32, 8, false, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
     rec_bwd_kernel<E, 16, 32, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
+  } else if (p.kind == REC_SLIM) {
+    rec_bwd_kernel<E, 4, 16, 4, PART><<<per, 64, 0, s>>>(a);
+  } else if (p.kind == REC_SLIM_LONG) {
+    if (p.segs > 1) rec_sum_kernel<E, 4, 128, 8, false, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
+    rec_bwd_kernel<E, 4, 128, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
   } else {
     if (p.segs > 1) rec_sum_kernel<E, 32, 16, 8, false, PART><<<per * (p.segs - 1), 512, 0, s>>>(a);
     rec_bwd_kernel<E, 32, 16, 8, PART><<<per * p.segs, 512, 0, s>>>(a);
@@ -878,7 +910,7 @@ int rec_step(hipStream_t s, const RecArgs& a, float* new_state) {
   return rs_status_after_launch();
 }
 
-// a wave's 64 steps of 2^23 elements of 4 bytes: 2^31 bytes, which a lane's offset holds
+// a wave's 128 steps (SLIM_LONG) of 2^23 elements: 2^32 bytes of fp32, which a lane's 32-bit offset holds
 bool rec_strides_ok(int64_t a, int64_t b, int64_t c) {
   return a < (1 << 23) && b < (1 << 23) && c < (1 << 23);
 }

@@ -378,6 +378,52 @@ def test_recurrence_segments_that_end_anywhere(B, T, D):
             assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("ragged", [False, True], ids=["", "ragged"])
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("B,T,D", [(3, 9, 1), (5, 33, 16), (4, 64, 17), (2, 65, 32), (7, 128, 3), (3, 129, 8), (300, 200, 12),
+                                   (260, 513, 9), (1, 1023, 16), (2, 1024, 31), (1, 1025, 7), (130, 2100, 2), (2, 9000, 10),
+                                   (150, 600, 40), (90, 600, 130)])
+def test_gated_recurrence_narrow(B, T, D, dtype, ragged):
+    """Few channels: one or two tiles of 32 bytes, with and without a cut time axis, and widths just above."""
+    test_gated_recurrence(B, T, D, dtype, ragged)
+
+
+def test_narrow_segments_that_end_anywhere():
+    """Narrow rows over a cut time axis: the same bits every time, the gradients of the joint input's halves."""
+    B, T, D = 2, 7000, 14
+    vg, h0 = rnd(B, T, 2 * D).requires_grad_(), rnd(B, D).requires_grad_()
+    dh, dlast = rnd(B, T, D), rnd(B, D)
+    for ends in ((0, T), (1, 1023), (1024, 1025), (T - 1, 2048), (4096, 6144)):
+        lengths = torch.tensor(ends, device=DEV)
+        h, last = gated_recurrence(vg, None, h0, lengths)
+        dvg, dh0 = torch.autograd.grad((h, last), (vg, h0), (dh, dlast))
+        want = ref_rec(vg.detach()[..., :D], vg.detach()[..., D:], h0.detach(), lengths, dh, dlast)
+        got = (h, last, dvg[..., :D], dvg[..., D:], dh0)
+        for a, (w, b), what in zip(got, want, ("h", "last", "dv", "dg", "dh0")):
+            near(a, w, b, f"{what} with ends {ends}")
+        for _ in range(3):
+            h, last = gated_recurrence(vg, None, h0, lengths)
+            dvg, dh0 = torch.autograd.grad((h, last), (vg, h0), (dh, dlast))
+            assert all(torch.equal(a, b) for a, b in zip(got, (h, last, dvg[..., :D], dvg[..., D:], dh0)))
+
+
+@pytest.mark.parametrize("T", [70, 130])
+def test_narrow_rows_far_apart(T):
+    """Steps 2^23 - 1 elements apart, which is as far as is taken: a wave's offsets come near 2^32 bytes."""
+    D, far = 8, 2 ** 23 - 1
+    big = torch.empty(1, T, far, device=DEV)
+    v, g = big[..., far - D:], big[..., 3:3 + D]
+    v.copy_(rnd(1, T, D))
+    g.copy_(rnd(1, T, D, mean=1.0))
+    dh = rnd(1, T, D)
+    apart = [t.detach().requires_grad_() for t in (v, g)]
+    dense = [t.detach().contiguous().requires_grad_() for t in (v, g)]
+    assert apart[0].stride(1) == far and dense[0].stride(1) == D
+    for a, b in zip(*((h, last, *torch.autograd.grad(h, leaves, dh))
+                      for leaves in (apart, dense) for h, last in (gated_recurrence(*leaves),))):
+        assert torch.equal(a, b)
+
+
 def test_recurrence_partial_arguments():
     """No state before, one output's gradient only, the joint form, int64 and odd lengths, strides."""
     B, T, D = 3, 70, 24
