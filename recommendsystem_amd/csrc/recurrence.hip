@@ -834,6 +834,10 @@ RecPlan rec_plan(int dtype, int64_t B, int64_t T, int D) {
   return p;
 }
 
+// Whether the backward starts a tile from a kept state rather than from h0.  SLIM_LONG keeps that of its
+// only tile too (B D floats): a backward of long rows without states is refused whatever their width.
+bool rec_keeps_states(const RecPlan& p) { return p.tiles > 1 || p.kind == REC_SLIM_LONG; }
+
 void rec_fill(RecArgs& a, const RecPlan& p, int64_t B, int64_t T, int D) {
   a.B = B;
   a.T = T;
@@ -925,8 +929,8 @@ bool rec_shape_ok(int dtype, int64_t B, int64_t T, int D) {
 
 RS_API int64_t rs_gated_rec_states_floats(int dtype, int64_t B, int64_t T, int D) {
   if (!rec_shape_ok(dtype, B, T, D)) return 0;
-  const int64_t tiles = rec_plan(dtype, B, T, D).tiles;
-  return tiles > 1 ? B * tiles * D : 0;
+  const RecPlan p = rec_plan(dtype, B, T, D);
+  return rec_keeps_states(p) ? B * p.tiles * D : 0;
 }
 
 RS_API int64_t rs_gated_rec_workspace_floats(int dtype, int64_t B, int64_t T, int D) {
@@ -952,7 +956,7 @@ RS_API int rs_gated_rec_fwd(void* stream, int dtype, const void* v, int64_t v_sb
   a.v = v, a.v_sb = v_sb, a.v_st = v_st;
   a.g = g, a.g_sb = g_sb, a.g_st = g_st;
   a.lengths = lengths, a.h0 = h0, a.h = h, a.last = last, a.ws = workspace;
-  a.states = p.tiles > 1 ? states : nullptr;
+  a.states = rec_keeps_states(p) ? states : nullptr;
   return RS_DISPATCH_ELEM(dtype, rec_fwd, rs_stream(stream), p, a);
 }
 
