@@ -824,9 +824,9 @@ RecPlan rec_plan(int dtype, int64_t B, int64_t T, int D) {
   p.tiles = (T + p.steps - 1) / p.steps;
   p.segs = 1;
   p.tps = (int)p.tiles;
-  const int64_t blocks = B * p.nct;
+  const int64_t blocks = B * p.nct;  // 0 for an empty batch, which has nothing to cut
   const bool cut = p.kind == REC_LONG || p.kind == REC_WIDE || p.kind == REC_SLIM_LONG;
-  if (cut && blocks <= 128 && p.tiles > 1) {
+  if (cut && blocks > 0 && blocks <= 128 && p.tiles > 1) {
     const int64_t want = 256 / blocks;
     p.tps = (int)((p.tiles + want - 1) / want);
     p.segs = (int)((p.tiles + p.tps - 1) / p.tps);

@@ -460,6 +460,16 @@ def test_recurrence_partial_arguments():
     assert not h.any() and torch.equal(last, s)
 
 
+@pytest.mark.parametrize("T,D", [(300, 24), (2000, 8), (5000, 1024)])
+def test_recurrence_of_an_empty_batch(T, D):
+    """Histories of more than one tile, but none of them: forward and backward of every long form."""
+    leaves = [rnd(0, T, D).requires_grad_(), rnd(0, T, D).requires_grad_(), rnd(0, D).requires_grad_()]
+    h, last = gated_recurrence(*leaves, torch.zeros(0, device=DEV, dtype=torch.int32))
+    assert h.shape == (0, T, D) and last.shape == (0, D)
+    for t, grad in zip(leaves, torch.autograd.grad((h, last), leaves, (rnd(0, T, D), rnd(0, D)))):
+        assert grad.shape == t.shape
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=names)
 def test_recurrence_extreme_gates(dtype):
     """Gates wide open, shut, infinite: i = sigmoid(-g) keeps its own digits where f rounds to 1."""

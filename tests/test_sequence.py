@@ -113,6 +113,16 @@ def test_size_queries():
     assert lib.rs_layernorm_bwd_workspace_floats(-1, 5) == 0
 
 
+def test_size_queries_of_empty_batches():
+    """No sequence needs no state and no workspace, whatever the length and the width's form."""
+    lib = _lib.load()
+    for T in (0, 1, 9, 65, 129, 300, 2000, 5000, 1 << 20):
+        for D in (1, 8, 24, 128, 264, 1024, 5000):
+            for code in (0, 1, 2):
+                assert lib.rs_gated_rec_states_floats(code, 0, T, D) == 0
+                assert lib.rs_gated_rec_workspace_floats(code, 0, T, D) == 0
+
+
 def test_meta_shapes():
     m = dict(device="meta")
     x, p = E(4, 5, 300, dtype=BF16, **m), E(300, **m)
