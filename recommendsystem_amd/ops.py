@@ -330,11 +330,22 @@ def _(x, gamma, beta, epsilon):
     return x.new_empty(x.shape), gamma.new_empty(2, x.numel() // x.shape[-1])
 
 
+def _like(t, dtype, shape, what):
+    """t is read through its raw pointer: what it holds has to be what the kernel takes it for."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(t.shape)}")
+
+
 @custom_op("ctr::layer_norm_bwd", mutates_args=())
 def layer_norm_bwd(dy: Tensor, x: Tensor, gamma: Tensor, stats: Tensor) -> tuple[Tensor, Tensor]:
-    """(dx, [dgamma | dbeta] [2, D])."""
+    """(dx, [dgamma | dbeta] [2, D]) for dy of x's type and shape and the stats of ctr::layer_norm."""
+    code = sequence._check_norm(x, gamma, gamma, 1.0)
+    _like(dy, x.dtype, x.shape, "layer_norm_bwd: dy")
+    _like(stats, torch.float32, (2, x.numel() // x.shape[-1]), "layer_norm_bwd: stats")
     return _lib.run_on(_lib.device_index(dy, x, gamma, stats), sequence._norm_backward, dy, x, None, None,
-                       gamma, stats, packing.element_code(x, "layer_norm's input"), None, False)
+                       gamma, stats.contiguous(), code, None, False)
 
 
 @layer_norm_bwd.register_fake
@@ -383,14 +394,21 @@ def _(v, g, h0, lengths):
 
 @custom_op("ctr::gated_recurrence_bwd", mutates_args=())
 def gated_recurrence_bwd(dh: Tensor, dlast: Tensor, v: Tensor, g: Optional[Tensor],
-                         h0: Optional[Tensor], lengths: Optional[Tensor], states: Tensor) -> tuple[Tensor, Tensor, Tensor]:
-    """(dv, dg, dh0); with g None dv is the joint rows' gradient and dg is empty."""
+                         h0: Optional[Tensor], lengths: Optional[Tensor],
+                         states: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    """(dv, dg, dh0) for dh of v's type, fp32 dlast and the states of ctr::gated_recurrence; with g
+    None dv is the joint rows' gradient and dg is empty."""
+    code = sequence._check_rec(v, g, 3, "gated_recurrence_bwd")
     B, T, D = _rec_sizes(v, g)
+    sequence._check_state(h0, (B, D), "gated_recurrence_bwd: h0")
+    _like(dh, v.dtype, (B, T, D), "gated_recurrence_bwd: dh")
+    _like(dlast, torch.float32, (B, D), "gated_recurrence_bwd: dlast")
+    _like(states, torch.float32, (sequence._rec_sizes(code, B, T, D)[0],), "gated_recurrence_bwd: states")
+    lengths = sequence._check_lengths(lengths, B, T)
     dv, dg, dh0 = _lib.run_on(_lib.device_index(v, g, dh, dlast, h0, lengths, states),
                               sequence._rec_backward, v, g,
-                              h0.contiguous() if h0 is not None else None,
-                              sequence._check_lengths(lengths, B, T), states, dh, dlast, packing.element_code(v, "gated_recurrence's values"),
-                              True)
+                              h0.contiguous() if h0 is not None else None, lengths,
+                              states.contiguous(), dh, dlast, code, True)
     return dv, v.new_empty(0) if dg is None else dg, dh0
 
 

@@ -62,6 +62,49 @@ def test_no_cpu_fallback(call):
         call()
 
 
+NORM_BWD = dict(dy=(E, (3, 4)), x=(E, (3, 4)), gamma=(E, (4,)), stats=(E, (2, 3)))
+# (the first width of this length that keeps states)
+REC_BWD = dict(dh=(E, (2, 300, 40)), dlast=(E, (2, 40)), v=(E, (2, 300, 40)), g=(E, (2, 300, 40)), h0=(E, (2, 40)),
+               lengths=None, states=(E, (_lib.load().rs_gated_rec_states_floats(0, 2, 300, 40),)))
+
+
+@pytest.mark.parametrize("op, args, name, shape, dtype, error", [
+    ("layer_norm_bwd", NORM_BWD, "dy", (3, 4), BF16, TypeError),
+    ("layer_norm_bwd", NORM_BWD, "dy", (2, 4), F32, ValueError),
+    ("layer_norm_bwd", NORM_BWD, "x", (3, 4), F16, TypeError),
+    ("layer_norm_bwd", NORM_BWD, "x", (3, 4), F64, TypeError),
+    ("layer_norm_bwd", NORM_BWD, "gamma", (3,), F32, ValueError),
+    ("layer_norm_bwd", NORM_BWD, "gamma", (4,), BF16, TypeError),
+    ("layer_norm_bwd", NORM_BWD, "stats", (2, 2), F32, ValueError),
+    ("layer_norm_bwd", NORM_BWD, "stats", (2, 3), F16, TypeError),
+    ("gated_recurrence_bwd", REC_BWD, "dh", (2, 300, 40), F16, TypeError),
+    ("gated_recurrence_bwd", REC_BWD, "dh", (2, 299, 40), F32, ValueError),
+    ("gated_recurrence_bwd", REC_BWD, "dlast", (2, 40), BF16, TypeError),
+    ("gated_recurrence_bwd", REC_BWD, "dlast", (1, 40), F32, ValueError),
+    ("gated_recurrence_bwd", REC_BWD, "g", (2, 300, 40), BF16, TypeError),
+    ("gated_recurrence_bwd", REC_BWD, "g", (2, 300, 39), F32, ValueError),
+    ("gated_recurrence_bwd", REC_BWD, "h0", (2, 39), F32, ValueError),
+    ("gated_recurrence_bwd", REC_BWD, "h0", (2, 40), F16, TypeError),
+    ("gated_recurrence_bwd", REC_BWD, "lengths", (3,), torch.int32, ValueError),
+    ("gated_recurrence_bwd", REC_BWD, "lengths", (2,), F32, TypeError),
+    ("gated_recurrence_bwd", REC_BWD, "states", (79,), F32, ValueError),
+    ("gated_recurrence_bwd", REC_BWD, "states", (0,), F32, ValueError),
+    ("gated_recurrence_bwd", REC_BWD, "states", (160,), BF16, TypeError),
+])
+def test_backward_operators_refuse_what_does_not_fit(op, args, name, shape, dtype, error):
+    """They read every argument through its raw pointer, with sizes taken from one of them."""
+    made = {k: a and a[0](*a[1]) for k, a in args.items()}
+    made[name] = E(shape, dtype=dtype)
+    with pytest.raises(error):
+        getattr(torch.ops.ctr, op)(*made.values())
+
+
+@pytest.mark.parametrize("op, args", [("layer_norm_bwd", NORM_BWD), ("gated_recurrence_bwd", REC_BWD)])
+def test_backward_operators_take_what_fits(op, args):
+    with pytest.raises(_lib.RecsysKernelError, match="ROCm device"):  # the next check after the sizes
+        getattr(torch.ops.ctr, op)(*(a and a[0](*a[1]) for a in args.values()))
+
+
 def test_lengths_checks():
     for bad, err in ((E(3), TypeError), (E(4, dtype=torch.int32), ValueError),
                      (E(3, 1, dtype=torch.int32), ValueError)):
