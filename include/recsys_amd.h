@@ -888,7 +888,7 @@ int rs_layernorm_bwd(void* stream, int dtype, const void* dy, int64_t ld_dy, con
 /* h_t = f_t h_{t-1} + (1 - f_t) v_t, f_t = sigmoid(g_t), for v, g [B, T, D] (batch stride *_sb,
  * step stride *_st).  h0 [B, D] (NULL: zeros).  lengths int32 [B] (NULL: T everywhere; values are
  * taken into 0..T): steps behind them are not read, h is zero there and the state stands still.
- * D and step strides (*_st) of 2^23 elements or more: -2.
+ * D and, with more than one step, step strides (*_st) of 2^23 elements or more: -2.
  * h [B, T, D] contiguous; last [B, D]: the state after lengths[b] steps.  states
  * (rs_gated_rec_states_floats, 0 for short sequences; NULL without a backward): fp32 states at
  * fixed steps, for rs_gated_rec_bwd with the same shape.  workspace: rs_gated_rec_workspace_floats floats. */

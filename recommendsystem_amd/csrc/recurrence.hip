@@ -914,9 +914,10 @@ int rec_step(hipStream_t s, const RecArgs& a, float* new_state) {
   return rs_status_after_launch();
 }
 
-// a wave's 128 steps (SLIM_LONG) of 2^23 elements: 2^32 bytes of fp32, which a lane's 32-bit offset holds
-bool rec_strides_ok(int64_t a, int64_t b, int64_t c) {
-  return a < (1 << 23) && b < (1 << 23) && c < (1 << 23);
+// a wave's 128 steps (SLIM_LONG) of 2^23 elements: 2^32 bytes of fp32, which a lane's 32-bit offset holds.
+// The step stride of a single step is never used.
+bool rec_strides_ok(int64_t T, int64_t a, int64_t b, int64_t c, int D) {
+  return D < (1 << 23) && (T <= 1 || (a < (1 << 23) && b < (1 << 23) && c < (1 << 23)));
 }
 
 // what the launches index: workgroups and time tiles in 31 bits
@@ -947,7 +948,7 @@ RS_API int rs_gated_rec_fwd(void* stream, int dtype, const void* v, int64_t v_sb
   if (B == 0) return RS_OK;
   if (!last || (T > 0 && (!v || !g || !h || v_sb < 0 || v_st < 0 || g_sb < 0 || g_st < 0)))
     return RS_ERR_ARG;
-  if (!rec_strides_ok(v_st, g_st, D)) return RS_ERR_UNSUPPORTED;
+  if (!rec_strides_ok(T, v_st, g_st, 0, D)) return RS_ERR_UNSUPPORTED;
   const int64_t need = rs_gated_rec_workspace_floats(dtype, B, T, D);
   if (need > 0 && (!workspace || workspace_floats < need)) return RS_ERR_ARG;
   const RecPlan p = rec_plan(dtype, B, T, D);
@@ -975,7 +976,8 @@ RS_API int rs_gated_rec_bwd(void* stream, int dtype, const void* v, int64_t v_sb
   if (T == 0 && !dh0) return RS_OK;
   const bool kept = rs_gated_rec_states_floats(dtype, B, T, D) > 0;
   if (kept && !states) return RS_ERR_ARG;
-  if (!rec_strides_ok(v_st, g_st, dh_st) || !rec_strides_ok(dv_st, dg_st, D)) return RS_ERR_UNSUPPORTED;
+  if (!rec_strides_ok(T, v_st, g_st, dh_st, D) || !rec_strides_ok(T, dv_st, dg_st, 0, D))
+    return RS_ERR_UNSUPPORTED;
   const int64_t need = rs_gated_rec_workspace_floats(dtype, B, T, D);
   if (need > 0 && (!workspace || workspace_floats < need)) return RS_ERR_ARG;
   const RecPlan p = rec_plan(dtype, B, T, D);

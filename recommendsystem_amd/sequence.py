@@ -183,11 +183,14 @@ MAX_STEP_STRIDE = 2 ** 23  # elements between two steps (and of a step) that the
 
 def _strided(t):
     """t [B, T, D] as the kernels read it, and its batch and step strides: in place with unit stride
-    along D and steps not too far apart, a contiguous copy otherwise."""
+    along D and steps not too far apart, a contiguous copy otherwise.  A single step has no next one:
+    whatever its stride says (a view of time-major rows may say anything) is not passed on."""
     sb, st, sc = t.stride()
+    if t.shape[1] <= 1:
+        st = 0
     if (sc != 1 and t.shape[2] != 1) or st >= MAX_STEP_STRIDE:
         t = t.contiguous()
-        sb, st, sc = t.stride()
+        sb, st, _ = t.stride()
     return t, sb, st
 
 

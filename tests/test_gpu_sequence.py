@@ -460,6 +460,31 @@ def test_recurrence_partial_arguments():
     assert not h.any() and torch.equal(last, s)
 
 
+def test_single_steps_of_time_major_rows():
+    """One step of [1, B, D] rows seen as [B, 1, D], 2^23 elements "to the next step", with a gradient
+    laid out likewise; through Python and through the C entries with the stride as it is."""
+    from recommendsystem_amd import _lib
+    B, D = 2 ** 13, 2 ** 10
+    v, g, dh = (rnd(1, B, D, dtype=torch.bfloat16).transpose(0, 1) for _ in range(3))
+    h0 = rnd(B, D)
+    far = v.stride(1)
+    assert far == 2 ** 23
+    leaves = [t.requires_grad_() for t in (v, g, h0)]
+    h, last = gated_recurrence(*leaves)
+    got = (h, last, *torch.autograd.grad(h, leaves, dh))
+    for a, (w, b), what in zip(got, ref_rec(v.detach(), g.detach(), h0.detach(), None, dh),
+                               ("h", "last", "dv", "dg", "dh0")):
+        near(a, w, b, what)
+    outs = [torch.empty_like(t) for t in got]
+    s = torch.cuda.current_stream().cuda_stream
+    p = [t.data_ptr() for t in (v, g, h0, *outs)]
+    _lib.call("rs_gated_rec_fwd", s, 1, p[0], D, far, p[1], D, far, B, 1, D, None, p[2], p[3], p[4], None, None, 0)
+    _lib.call("rs_gated_rec_bwd", s, 1, p[0], D, far, p[1], D, far, B, 1, D, None, p[2], None, dh.data_ptr(), D,
+              far, None, p[5], D, far, p[6], D, far, p[7], None, 0)
+    for a, b in zip(outs, got):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("T,D", [(300, 24), (2000, 8), (5000, 1024)])
 def test_recurrence_of_an_empty_batch(T, D):
     """Histories of more than one tile, but none of them: forward and backward of every long form."""

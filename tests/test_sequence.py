@@ -114,6 +114,23 @@ def test_lengths_checks():
     assert got.dtype == torch.int32 and got.tolist() == [5, 0, 3]
 
 
+def test_strides_of_a_single_step():
+    """A [B, 1, D] view of time-major [1, B, D] rows says B D elements to the next step, and counts as
+    contiguous: there is no next step, so nothing has to be copied and nothing is refused."""
+    far = E(1, 8192, 1024, device="meta").transpose(0, 1)
+    assert far.stride(1) >= sequence.MAX_STEP_STRIDE
+    t, sb, st = sequence._strided(far)
+    assert t is far and sb == 1024 and st < sequence.MAX_STEP_STRIDE
+    two = E(2, 8192, 1024, device="meta").transpose(0, 1)      # with a next step it is copied
+    assert sequence._strided(two)[1:] == (2048, 1024)
+    # the C entries: a step stride that is too long is refused where there are two steps
+    lib, p, far = _lib.load(), torch.zeros(64).data_ptr(), 1 << 23
+    UNS = _lib.RS_ERR_UNSUPPORTED
+    assert lib.rs_gated_rec_fwd(None, 0, p, 4, far, p, 4, 4, 1, 2, 4, None, None, p, p, None, None, 0) == UNS
+    assert lib.rs_gated_rec_bwd(None, 0, p, 4, 4, p, 4, 4, 1, 2, 4, None, None, None, p, 4, far, p, p, 4, 4, p,
+                                4, 4, p, None, 0) == UNS
+
+
 def test_entry_points_reject():
     """The C entry points refuse what they cannot run before they launch (null or short buffers)."""
     lib = _lib.load()
