@@ -22,6 +22,7 @@ import functools
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -40,6 +41,15 @@ def _first_order(backward):
     return staticmethod(lambda ctx, *g: once(ctx, *g) if torch.is_grad_enabled() else backward(ctx, *g))
 
 
+def _refuse_tangents(what, *tensors):
+    """There is no forward-mode derivative: a dual tensor is refused, its tangent would be lost."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual level is open (0.3 us a tensor less)
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative (jvp)")
+
+
 # sizes that follow from a shape alone
 @functools.lru_cache(maxsize=1024)
 def _norm_workspace(R, D):
@@ -56,6 +66,7 @@ def _rec_sizes(code, B, T, D):
 # layer normalisation
 # ============================================================================================
 def _check_norm(x, gamma, beta, epsilon):
+    _refuse_tangents("layer_norm", x, gamma, beta)
     code = element_code(x, "layer_norm's input")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
         raise ValueError(f"layer_norm needs a last dimension of 1 to {MAX_WIDTH}, got shape "
@@ -203,6 +214,7 @@ def _halves(v, g):
 
 
 def _check_rec(v, g, dims, what):
+    _refuse_tangents(what, v, g)
     if v.dim() != dims:
         raise ValueError(f"{what} takes rank-{dims} values, got shape {tuple(v.shape)}")
     code = element_code(v, f"{what}'s values")
@@ -232,6 +244,7 @@ def _any_grad(*tensors):
 def _check_state(state, shape, what):
     if state is None:
         return
+    _refuse_tangents(what, state)
     if state.dtype is not torch.float32:
         raise TypeError(f"{what} must be float32, got {state.dtype}")
     if state.shape != shape:

@@ -105,6 +105,40 @@ def test_backward_operators_take_what_fits(op, args):
         getattr(torch.ops.ctr, op)(*(a and a[0](*a[1]) for a in args.values()))
 
 
+def dual(*shape):
+    return torch.autograd.forward_ad.make_dual(torch.ones(*shape), torch.ones(*shape))
+
+
+@pytest.mark.parametrize("call", [
+    lambda: sequence.layer_norm(dual(3, 4), E(4), E(4)),
+    lambda: sequence.layer_norm(E(3, 4), dual(4), E(4), save_8bit=True),
+    lambda: sequence.layer_norm(E(3, 4), E(4), dual(4)),
+    lambda: sequence.gated_recurrence(dual(2, 3, 4), E(2, 3, 4)),
+    lambda: sequence.gated_recurrence(E(2, 3, 4), dual(2, 3, 4)),
+    lambda: sequence.gated_recurrence(dual(2, 3, 4)),
+    lambda: sequence.gated_recurrence(E(2, 3, 4), E(2, 3, 4), dual(2, 4)),
+    lambda: sequence.gated_recurrence_step(dual(2, 4), E(2, 4)),
+    lambda: sequence.gated_recurrence_step(E(2, 4), E(2, 4), dual(2, 4)),
+    lambda: torch.ops.ctr.layer_norm(dual(3, 4), E(4), E(4), 1e-5),
+    lambda: torch.ops.ctr.gated_recurrence(dual(2, 3, 4), None, None, None),
+])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(call, grad):
+    """Not dropped: without a jvp the output would come back with no tangent and no word."""
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(NotImplementedError, match="jvp"):
+            call()
+
+
+def test_tangents_of_others_do_not_matter():
+    with pytest.raises(NotImplementedError, match="jvp"):
+        torch.func.jvp(lambda x: sequence.layer_norm(x, E(4), E(4)), (E(3, 4),), (E(3, 4),))
+    with torch.autograd.forward_ad.dual_level():
+        dual(3, 4)
+        with pytest.raises(_lib.RecsysKernelError, match="ROCm device"):
+            sequence.layer_norm(E(3, 4), E(4), E(4))
+
+
 def test_lengths_checks():
     for bad, err in ((E(3), TypeError), (E(4, dtype=torch.int32), ValueError),
                      (E(3, 1, dtype=torch.int32), ValueError)):
