@@ -352,7 +352,7 @@ class Dense(nn.Module):
             self.build(tuple(x.shape), device=x.device)
         lead = x.shape[:-1]  # Keras Dense = tensordot over the last axis
         from . import ops
-        if ops.custom_ops_enabled() and not self.save_8bit:
+        if ops.custom_ops_enabled() and not (self.save_8bit and torch.is_grad_enabled()):
             y = torch.ops.ctr.dense(x.reshape(-1, x.shape[-1]).float(), self.kernel, self.bias, self.act)
             return y.reshape(*lead, self.units)
         y = _DenseFn.apply(x.reshape(-1, x.shape[-1]).float(), self.kernel, self.bias, self.act,

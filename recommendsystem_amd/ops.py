@@ -15,11 +15,13 @@ kernels:
                                                   (embedding.SparseTable), not an autograd output
     ctr::layer_norm / ctr::layer_norm_bwd         sequence.layer_norm
     ctr::gated_recurrence / _bwd                  sequence.gated_recurrence
+    ctr::gated_recurrence_step                    sequence.gated_recurrence_step (no autograd formula)
     ctr::pack8 / ctr::unpack8                     packing.pack8 / unpack8 (no autograd formula)
 
 The layer classes (layers.InteractingLayer, din.DIN, layers.Dense) keep their in-place gradient
 fast path (autograd.Function writing into the flat parameter block); ``use_custom_ops(True)``
-routes them through these ops instead (functional gradients; traceable).
+routes them through these ops instead (functional gradients; traceable), and with them the sequence
+operators, with and without gradients.  Training with ``save_8bit`` has no traced form.
 """
 from __future__ import annotations
 
@@ -37,7 +39,7 @@ _USE = _lib.CUSTOM_OPS
 
 
 def use_custom_ops(on: bool = True) -> None:
-    """Route InteractingLayer / DIN / Dense forward through torch.ops.ctr (traceable)."""
+    """Route InteractingLayer / DIN / Dense / the sequence operators through torch.ops.ctr (traceable)."""
     _USE["on"] = bool(on)
 
 
@@ -431,6 +433,21 @@ def _rec_op_backward(ctx, dh, dlast, _dstates):
 
 
 gated_recurrence.register_autograd(_rec_op_backward, setup_context=_rec_setup)
+
+
+@custom_op("ctr::gated_recurrence_step", mutates_args=())
+def gated_recurrence_step(v: Tensor, g: Optional[Tensor], state: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    """(h, the new state) of sequence.gated_recurrence_step."""
+    code = sequence._check_rec(v, g, 2, "gated_recurrence_step")
+    B, D = v.shape if g is not None else (v.shape[0], v.shape[1] // 2)
+    sequence._check_state(state, (B, D), "gated_recurrence_step: state")
+    return _lib.run_on(_lib.device_index(v, g, state), sequence._rec_step, v, g, state, None, B, D, code)
+
+
+@gated_recurrence_step.register_fake
+def _(v, g, state):
+    B, D = v.shape if g is not None else (v.shape[0], v.shape[1] // 2)
+    return v.new_empty(B, D), v.new_empty(B, D, dtype=torch.float32)
 
 
 @custom_op("ctr::pack8", mutates_args=())

@@ -143,9 +143,10 @@ class _LayerNormFn(torch.autograd.Function):
 def _norm(x, gamma, beta, epsilon, save_8bit, in_place):
     code = _check_norm(x, gamma, beta, epsilon)
     index = device_index(x, gamma, beta)
-    if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
-        if _lib.CUSTOM_OPS["on"] and not save_8bit:
-            return torch.ops.ctr.layer_norm(x, gamma, beta, epsilon)[0]
+    train = torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad)
+    if _lib.CUSTOM_OPS["on"] and not (train and save_8bit):
+        return torch.ops.ctr.layer_norm(x, gamma, beta, epsilon)[0]
+    if train:
         return _LayerNormFn.apply(x, gamma, beta, epsilon, code, save_8bit, in_place, index)
     return run_on(index, _norm_forward, x, gamma, beta, epsilon, code, False, False)[0]
 
@@ -336,11 +337,11 @@ def gated_recurrence(v, g=None, h0=None, lengths=None):
     _check_state(h0, (B, D), "gated_recurrence: h0")
     index = device_index(v, g, h0, lengths)
     lengths = _check_lengths(lengths, B, T)
+    if _lib.CUSTOM_OPS["on"]:
+        return tuple(torch.ops.ctr.gated_recurrence(v, g, h0, lengths)[:2])
     if h0 is not None:
         h0 = h0.contiguous()
     if torch.is_grad_enabled() and _any_grad(v, g, h0):
-        if _lib.CUSTOM_OPS["on"]:
-            return tuple(torch.ops.ctr.gated_recurrence(v, g, h0, lengths)[:2])
         return _RecurrenceFn.apply(v, g, h0, lengths, code, index)
     return run_on(index, _rec_forward, v, g, h0, lengths, code, False)[:2]
 
@@ -359,7 +360,11 @@ def gated_recurrence_step(v, g=None, state=None, out=None):
     if torch.is_grad_enabled() and _any_grad(v, g, state, out):
         raise RuntimeError("gated_recurrence_step has no backward: call it under torch.no_grad(), or "
                            "gated_recurrence with one step")
-    return run_on(device_index(v, g, state, out), _rec_step, v, g, state, out, B, D, code)
+    index = device_index(v, g, state, out)
+    if _lib.CUSTOM_OPS["on"]:
+        h, new = torch.ops.ctr.gated_recurrence_step(v, g, state)
+        return h, new if out is None else out.copy_(new)
+    return run_on(index, _rec_step, v, g, state, out, B, D, code)
 
 
 def _rec_step(v, g, state, out, B, D, code, stream):

@@ -814,3 +814,31 @@ def test_custom_operators():
     finally:
         ops.use_custom_ops(False)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_custom_operators_without_gradients():
+    """Inference through the operators: the same bits as without them; the step in place as well."""
+    from recommendsystem_amd import ops
+    x, g = rnd(3, 300, 40), rnd(3, 300, 40)
+    gamma, beta, h0 = rnd(40), rnd(40), rnd(3, 40)
+    lengths = torch.tensor([300, 0, 77], device=DEV)
+    enc = SequenceEncoder(16, depth=2, save_8bit=True)
+    for op, args in ((torch.ops.ctr.gated_recurrence_step, (x[:, 0], g[:, 0], h0)),
+                     (torch.ops.ctr.gated_recurrence_step, (x[:, 0], None, None))):
+        torch.library.opcheck(op.default, args)
+
+    def run():
+        state = h0.clone()
+        h, new = gated_recurrence_step(x[:, 0], g[:, 0], state, state)
+        assert new is state
+        with torch.no_grad():
+            y, states = enc(x, lengths)
+            return (layer_norm(x, gamma, beta), *gated_recurrence(x, g, h0, lengths), h, new, y, states,
+                    *enc.step(x[:, 1], states))
+    want = run()
+    ops.use_custom_ops(True)
+    try:
+        got = run()
+    finally:
+        ops.use_custom_ops(False)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

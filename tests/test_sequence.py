@@ -233,6 +233,42 @@ def test_meta_shapes():
     assert torch.ops.ctr.unpack8(codes, scales, F16).dtype == F16
 
 
+@pytest.fixture
+def custom_ops():
+    ops.use_custom_ops(True)
+    yield
+    ops.use_custom_ops(False)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_traced_without_a_device(custom_ops, grad):
+    """The functions over fake tensors, with gradients wanted and without (nothing is launched)."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(), torch.set_grad_enabled(grad):
+        x, p, s = (E(*shape, device="cuda", requires_grad=grad) for shape in ((4, 300, 40), (40,), (4, 40)))
+        assert sequence.layer_norm(x, p, p).shape == x.shape
+        for g in (x, None):
+            h, last = sequence.gated_recurrence(x, g, s if g is not None else None)
+            assert h.shape == (4, 300, 40 if g is not None else 20) and last.shape == (4, h.shape[2])
+    with FakeTensorMode():
+        v, s = E(4, 40, device="cuda", dtype=BF16), E(4, 40, device="cuda")
+        h, new = sequence.gated_recurrence_step(v, v, s, s)
+        assert new is s and h.shape == v.shape and h.dtype == BF16
+        assert sequence.gated_recurrence_step(v)[1].shape == (4, 20)
+
+
+@pytest.mark.parametrize("save_8bit", [False, True])
+def test_encoder_traced_for_serving(custom_ops, save_8bit):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(), torch.no_grad():
+        enc = sequence.SequenceEncoder(16, depth=2, save_8bit=save_8bit)
+        lengths = E(3, device="cuda", dtype=torch.int64)
+        y, states = enc(E(3, 70, 24, device="cuda"), lengths)
+        assert y.shape == (3, 70, 24) and states.shape == (2, 3, 16)
+        y, states = enc.step(E(3, 24, device="cuda"), states)
+        assert y.shape == (3, 24) and states.shape == (2, 3, 16)
+
+
 def test_dense_flag_defaults_off():
     assert not Dense(3).save_8bit and Dense(3, save_8bit=True).save_8bit
     assert packing.scale_shape((2, 129)) == (2, 2)
