@@ -2,10 +2,11 @@
 //   mean = sum x / D, rstd = 1 / sqrt(sum (x - mean)^2 / D + eps), xh = (x - mean) rstd
 //   y = xh gamma + beta
 //   w = dy gamma;  dx = rstd (w - mean(w) - xh mean(w xh));  dgamma = sum_rows dy xh;  dbeta = sum_rows dy
-// All sums are held in fp32.  The forward sums x - x[0] and the mean is corrected by the mean of x -
-// mean, in both passes (both subtract without error when the row's spread is small against its
-// offset), so a row with a large offset loses nothing to the rounding of its own mean, and a
-// constant row is normalised to exact zeros.
+// All sums are held in fp32.  The forward takes a first mean m = x[0] + mean(x - x[0]), and both
+// passes correct it by the mean of x - m (both differences have no error when the row's spread is
+// small against its offset), so a row with a large offset loses nothing to the rounding of its own
+// mean, and a constant row is normalised to exact zeros.  x[0] serves for m alone: the differences that
+// are kept are those of x itself from m, so a first column far off the others costs them no digits.
 //
 // Bound by memory.  A row lives in the registers of TPR threads (1 .. 64 lanes of a wave, or 2 to 8
 // waves), NCH x 16 bytes each, so it is read once; workgroups stay and walk the rows, with gamma and
@@ -133,19 +134,16 @@ __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_fwd_kernel(const LnA
     for (int c = 0; c < NCH; ++c) {
       const int nv = a.D - (c * TPR + tr) * V;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        x[c][j] -= x0;
-        s[0] += j < nv ? x[c][j] : 0.f;
-      }
+      for (int j = 0; j < V; ++j) s[0] += j < nv ? x[c][j] - x0 : 0.f;
     }
     row_sum<1, TPR>(s, red, flip);
-    const float m0 = s[0] * inv;
+    const float m = fmaf(s[0], inv, x0);
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int nv = a.D - (c * TPR + tr) * V;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        x[c][j] = j < nv ? x[c][j] - m0 : 0.f;
+        x[c][j] = j < nv ? x[c][j] - m : 0.f;
         q[0] += x[c][j];
         q[1] = fmaf(x[c][j], x[c][j], q[1]);
       }
@@ -164,7 +162,7 @@ __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_fwd_kernel(const LnA
         if (col < a.D) store16<E>((X*)a.y + row * a.ldy + col, y, a.D - col);
       }
       if (tr == 0 && a.mean) {
-        a.mean[row] = x0 + (m0 + dl);
+        a.mean[row] = m + dl;
         a.rstd[row] = rs;
       }
     }
@@ -361,11 +359,11 @@ __global__ void __launch_bounds__(LN_WIDE) ln_wide_fwd_kernel(const LnArgs a) {
       for (int j = 0; j < V; ++j) s[0] += j < nv ? x[j] - x0 : 0.f;
     });
     row_sum<1, LN_WIDE>(s, red, flip);
-    const float m0 = s[0] / (float)D;
+    const float m = x0 + s[0] / (float)D;
     for_row<E>(xr, D, [&](const float* x, int, int nv) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = j < nv ? x[j] - x0 - m0 : 0.f;
+        const float d = j < nv ? x[j] - m : 0.f;
         q[0] += d;
         q[1] = fmaf(d, d, q[1]);
       }
@@ -378,11 +376,11 @@ __global__ void __launch_bounds__(LN_WIDE) ln_wide_fwd_kernel(const LnArgs a) {
       load_f<V>(gm, a.gamma + col, nv);
       load_f<V>(bt, a.beta + col, nv);
 #pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = fmaf((x[j] - x0 - m0 - dl) * rs, gm[j], bt[j]);
+      for (int j = 0; j < V; ++j) y[j] = fmaf((x[j] - m - dl) * rs, gm[j], bt[j]);
       store16<E>((X*)a.y + r * a.ldy + col, y, nv);
     });
     if (threadIdx.x == 0 && a.mean) {
-      a.mean[r] = x0 + (m0 + dl);
+      a.mean[r] = m + dl;
       a.rstd[r] = rs;
     }
     if (a.codes) {  // 32 lanes x 4 elements a block

@@ -200,6 +200,31 @@ def test_layer_norm_offset_constant_and_not_finite():
     assert not y[[0, 2, 4]].isnan().any()
 
 
+@pytest.mark.parametrize("save_8bit", [False, True], ids=["", "8bit"])
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("D", [2, 40, 300, 1024, 8192, 16385, 32768])
+@pytest.mark.parametrize("at", [0, -1])
+def test_layer_norm_outlier(at, D, dtype, save_8bit):
+    """One channel far above the others, as residual streams have them, the first one or the last: it
+    takes no digits from the others.  A sum is off by 48 u of its terms' magnitudes, the mean so by 48 u
+    of the mean |deviation|, which is far below the standard deviation here: 64 u (|xh| + mean |xh|)."""
+    x = rnd(3, D)
+    x[:, at] = 3e4 if dtype is torch.float16 else 1e6
+    x = x.to(dtype).requires_grad_()
+    gamma, beta = rnd(D, mean=1.0, std=0.2).requires_grad_(), rnd(D).requires_grad_()
+    dy = rnd(3, D, dtype=dtype)
+    y = layer_norm(x, gamma, beta, 1e-5, save_8bit)
+    grads = torch.autograd.grad(y, (x, gamma, beta), dy)
+    kept = unpacked(*ref_pack(x.detach().double().cpu())) if save_8bit else None
+    want = ref_norm(x.detach(), gamma, beta, 1e-5, dy, kept)
+    xd, gd = x.detach().double().cpu(), gamma.detach().double().cpu()
+    dev = xd - xd.mean(1, keepdim=True)
+    xh = dev.abs() / torch.sqrt(dev.pow(2).mean(1, keepdim=True) + 1e-5)
+    want[0] = want[0][0], 64 * U * (xh + xh.mean(1, keepdim=True)) * gd.abs() + 4 * U * beta.detach().double().cpu().abs()
+    for got, (w, bound), what in zip((y, *grads), want, ("y", "dx", "dgamma", "dbeta")):
+        near(got, w, bound, what)
+
+
 def test_layer_norm_strides_ranks_and_empty():
     gamma, beta = rnd(40, mean=1.0).requires_grad_(), rnd(40).requires_grad_()
     wide = rnd(12, 100)
