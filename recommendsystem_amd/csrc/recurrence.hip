@@ -1,9 +1,11 @@
 // Gated linear recurrence over [B, T, D] and its gradients, all channels independent:
 //   i_t = sigmoid(-g_t) = 1 - f_t        h_t = f_t h_{t-1} + (1 - f_t) v_t = h_{t-1} + i_t (v_t - h_{t-1})
 //   r_t = the gradient that reaches h_t from later steps, a_t = dh_t + r_t
-//   dv_t = i_t a_t     dg_t = a_t (h_{t-1} - v_t) i_t (1 - i_t)     r_{t-1} = a_t - i_t a_t
-// The state and its gradient are fp32 throughout.  Written with i rather than f: a gate that is
-// almost open (f rounds to 1) still moves the state by its own small i.
+//   dv_t = i_t a_t     dg_t = a_t (h_{t-1} - v_t) i_t f_t     r_{t-1} = f_t a_t
+// The state and its gradient are fp32 throughout.  A step is kept as the smaller one of i and f, to its
+// own digits, and the other one is never formed where it would round to 1: an almost open gate still
+// moves the state by its small i, an almost shut one still passes its small f of the state and of the
+// gradient.
 // Steps from lengths[b] on are not read: h, dv and dg are zero there and the state stands still.
 //
 // A run of steps takes the state in front of it, s, to A s + H: A = f_1 f_2 ... is what it keeps, H
@@ -54,12 +56,28 @@ struct RecArgs {
   float* ws;  // [segs][2][B D]: (A, H) of every segment
 };
 
+// A step's gate as one signed number: i for an open gate (g >= 0), -f for a shut one, with -0 where f
+// vanishes; at most 1/2 in magnitude, m.
 template <class E>
-__device__ __forceinline__ float rec_input_gate(float g) {
-  // exp = inf gives 0.  16-bit rows take the hardware's exp2 of the rounded g log2(e), off by |g| half
-  // steps of fp32 relative to the gate
-  return __builtin_amdgcn_rcpf(1.0f + (sizeof(typename E::T) == 4 ? expf(g) : __expf(g)));
+__device__ __forceinline__ float rec_gate(float g) {
+  // exp = inf gives i = 0.  16-bit rows take the hardware's exp2 of the rounded g log2(e), off by |g|
+  // half steps of fp32 relative to the gate; the reciprocal is off by one step
+  const float e = sizeof(typename E::T) == 4 ? expf(g) : __expf(g), i = __builtin_amdgcn_rcpf(1.0f + e);
+  return g < 0.f ? -(e * i) : i;
 }
+__device__ __forceinline__ bool gate_shut(float w) { return __float_as_int(w) < 0; }
+// The same gate of which the compiler does not know the sign: it tests it again, rather than keep a
+// lane mask for every step of a tile from one pass over the steps to the next.
+__device__ __forceinline__ float gate_again(float w) {
+  asm("" : "+v"(w));
+  return w;
+}
+// f s + i v, as s + i (v - s) or v + f (s - v); d = s - v
+__device__ __forceinline__ float gate_step(float w, bool shut, float s, float v, float d) {
+  return fmaf(-w, d, shut ? v : s);
+}
+// f x
+__device__ __forceinline__ float gate_keep(float w, bool shut, float x) { return fmaf(-w, x, shut ? 0.f : x); }
 
 // the bits of a gate that lets nothing in (+infinity), twice for 16-bit elements
 template <class E>
@@ -477,9 +495,10 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
       E::template unpack<2>(rv[k].w, v);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float i = in[k][j] = rec_input_gate<E>(g[j]);
-        H[j] = fmaf(i, v[j] - H[j], H[j]);
-        A[j] = fmaf(-i, A[j], A[j]);
+        const float w = in[k][j] = rec_gate<E>(g[j]);
+        const bool shut = g[j] < 0.f;
+        H[j] = gate_step(w, shut, H[j], v[j], H[j] - v[j]);
+        A[j] = gate_keep(w, shut, A[j]);
       }
     }
     if (a.states && p.grp == 0)
@@ -492,7 +511,7 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
       E::template unpack<2>(rv[k].w, v);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        st[j] = fmaf(in[k][j], v[j] - st[j], st[j]);
+        st[j] = gate_step(in[k][j], gate_shut(in[k][j]), st[j], v[j], st[j] - v[j]);
         o[j] = W || t + rh_.ls + k < p.n ? st[j] : 0.f;
       }
       if (W || t + rh_.ls + k < a.T) store8<E, PART>(rh_.at(t, k), o, p.nv);
@@ -568,10 +587,10 @@ __global__ void __launch_bounds__(LC * NG) rec_sum_kernel(const RecArgs a) {
       E::template unpack<2>(rx[k].w, x);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float i = rec_input_gate<E>(g[j]);
-        if (FWD) H[j] = fmaf(i, x[j] - H[j], H[j]);
-        else H[j] = fmaf(-i, x[j] + H[j], x[j] + H[j]);
-        A[j] = fmaf(-i, A[j], A[j]);
+        const float w = rec_gate<E>(g[j]);
+        const bool shut = g[j] < 0.f;
+        H[j] = FWD ? gate_step(w, shut, H[j], x[j], H[j] - x[j]) : gate_keep(w, shut, x[j] + H[j]);
+        A[j] = gate_keep(w, shut, A[j]);
       }
     }
   }
@@ -586,8 +605,9 @@ __global__ void __launch_bounds__(LC * NG) rec_sum_kernel(const RecArgs a) {
 // ---------------------------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------------------------
+// (two waves a SIMD: a register more than its 256 would leave the short forms one)
 template <class E, int LC, int NG, int K, bool PART>
-__global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
+__global__ void __launch_bounds__(LC * NG, 2) rec_bwd_kernel(const RecArgs a) {
   constexpr int V = VC<E>::V, STEPS = NG * K;
   typedef typename E::T X;
   __shared__ __attribute__((aligned(16))) float lds[2][ScanLds<LC, NG, V, 3>::FLOATS];
@@ -654,9 +674,10 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
       E::template unpack<2>(nv_[k].w, e[k]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float i = in[k][j] = rec_input_gate<E>(g[j]);
-        H[j] = fmaf(i, e[k][j] - H[j], H[j]);
-        A[j] = fmaf(-i, A[j], A[j]);
+        const float w = in[k][j] = rec_gate<E>(g[j]);
+        const bool shut = g[j] < 0.f;
+        H[j] = gate_step(w, shut, H[j], e[k][j], H[j] - e[k][j]);
+        A[j] = gate_keep(w, shut, A[j]);
       }
     }
 #pragma unroll
@@ -664,10 +685,7 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
       float d[V];
       E::template unpack<2>(rd[k].w, d);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float x = d[j] + G[j];
-        G[j] = fmaf(-in[k][j], x, x);
-      }
+      for (int j = 0; j < V; ++j) G[j] = gate_keep(in[k][j], gate_shut(in[k][j]), d[j] + G[j]);
     }
     next();
     tile_scan_both<LC, NG, V>(A, H, G, s, r, st, rt, lds[tile & 1]);
@@ -675,9 +693,9 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = st[j] - e[k][j];  // h_{t-1} - v_t
-        e[k][j] = d;
-        st[j] = fmaf(-in[k][j], d, st[j]);
+        const float w = in[k][j], v = e[k][j];
+        e[k][j] = st[j] - v;  // h_{t-1} - v_t
+        st[j] = gate_step(w, gate_shut(w), st[j], v, e[k][j]);
       }
 #pragma unroll
     for (int k = K - 1; k >= 0; --k) {
@@ -685,10 +703,12 @@ __global__ void __launch_bounds__(LC * NG) rec_bwd_kernel(const RecArgs a) {
       E::template unpack<2>(rd[k].w, d);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float i = in[k][j], x = d[j] + rt[j];
-        gv[j] = i * x;
-        gg[j] = gv[j] * e[k][j] * (1.0f - i);
-        rt[j] = x - gv[j];
+        // the smaller and the larger part of x, f x and i x or the other way round
+        const float w = gate_again(in[k][j]), m = fabsf(w), x = d[j] + rt[j], lo = m * x, hi = fmaf(-m, x, x);
+        const bool shut = gate_shut(w);
+        gv[j] = shut ? hi : lo;
+        gg[j] = m * hi * e[k][j];
+        rt[j] = shut ? lo : hi;
       }
       if (W || t + rdv_.ls + k < a.T) {
         store8<E, PART>(rdv_.at(t, k), gv, p.nv);
@@ -746,7 +766,7 @@ __global__ void __launch_bounds__(256) rec_step_kernel(const RecArgs a, float* n
   E::template unpack<2>(rv.w, v);
   E::template unpack<2>(rg.w, g);
 #pragma unroll
-  for (int j = 0; j < V; ++j) s[j] = fmaf(rec_input_gate<E>(g[j]), v[j] - s[j], s[j]);
+  for (int j = 0; j < V; ++j) s[j] = gate_step(rec_gate<E>(g[j]), g[j] < 0.f, s[j], v[j], s[j] - v[j]);
   store8<E, true>((X*)a.h + b * a.D + c0, s, nv);
   store_n<V, true>(new_state + b * a.D + c0, s, nv);
 }

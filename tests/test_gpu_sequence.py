@@ -535,6 +535,67 @@ def test_recurrence_extreme_gates(dtype):
             near(a, w, b + 1e-38, f"{what} at gate {gate}")
 
 
+def ref_shut(v, g, h0, dh, dlast):
+    """(value, bound) pairs as ref_rec's, for gates below 0 with every term of the bound scaled by its own
+    factor f or i: f = e^g / (1 + e^g) holds to gate = 12 u of itself (exponential, sum, reciprocal,
+    product), for 16-bit rows and 2 |g| u more (the rounded exponent of the hardware's exp2)."""
+    B, T, D = v.shape
+    gate = U * (12 + (2 * g.double().cpu().abs() if g.dtype != torch.float32 else torch.zeros(())))
+    gate = gate.expand(B, T, D)
+    v, g, s, dh, r = (t.double().cpu() for t in (v, g, h0, dh, dlast))
+    f, i = torch.sigmoid(g), torch.sigmoid(-g)
+    e, top = torch.zeros(B, D).double(), s.abs()
+    hs, es = [s], [e]
+    for t in range(T):
+        new = f[:, t] * s + i[:, t] * v[:, t]
+        e = f[:, t] * (e + (gate[:, t] + 8 * U) * top) + 8 * U * (i[:, t] * v[:, t].abs() + new.abs())
+        top = f[:, t] * top + i[:, t] * v[:, t].abs()
+        s = new
+        hs.append(s)
+        es.append(e)
+    H, EH = torch.stack(hs, 1), torch.stack(es, 1)
+    out = [(H[:, 1:], EH[:, 1:]), (s, e)]
+    er, big = torch.zeros(B, D).double(), r.abs()
+    dv, dg, bv, bg = (torch.zeros(B, T, D).double() for _ in range(4))
+    for t in range(T - 1, -1, -1):
+        a = r + dh[:, t]
+        ea = er + 8 * U * (a.abs() + r.abs())
+        d = H[:, t] - v[:, t]
+        dv[:, t], bv[:, t] = i[:, t] * a, i[:, t] * (ea + 8 * U * a.abs())
+        dg[:, t] = a * d * i[:, t] * f[:, t]
+        bg[:, t] = i[:, t] * f[:, t] * (ea * d.abs() + a.abs() * (EH[:, t] + U * d.abs())
+                                        + (gate[:, t] + 16 * U) * (a * d).abs())
+        big = f[:, t] * (big + dh[:, t].abs())
+        er = f[:, t] * ea + (gate[:, t] + 8 * U) * (f[:, t] * a.abs() + big)
+        r = f[:, t] * a
+    return out + [(dv, bv), (dg, bg), (r, er)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("B,T,D", [(2, 1, 24), (3, 5, 24), (2, 20, 130), (2, 60, 130), (2, 50, 8), (1, 300, 24), (2, 1100, 8),
+                                   (1, 6000, 24), (2, 700, 1000)])
+def test_recurrence_of_almost_shut_gates(B, T, D, dtype):
+    """f = sigmoid(g) down to e^-30 keeps its own digits: the little of a large state that passes, the
+    gradient that reaches it, and the gates' own gradients."""
+    v, dh = rnd(B, T, D, dtype=dtype), rnd(B, T, D, dtype=dtype)
+    g = (-4 - 26 * torch.rand(B, T, D, device=DEV)).to(dtype)
+    h0, dlast = 1e5 * rnd(B, D), 1e5 * rnd(B, D)
+    leaves = [t.clone().requires_grad_() for t in (v, g, h0)]
+    h, last = gated_recurrence(*leaves)
+    got = (h, last, *torch.autograd.grad((h, last), leaves, (dh, dlast)))
+    for a, (w, b), what in zip(got, ref_shut(v, g, h0, dh, dlast), ("h", "last", "dv", "dg", "dh0")):
+        if dtype is torch.float16 and a.dtype == dtype:
+            # dlast times i passes fp16's largest number, 65504: from 65520 on the nearest is infinity
+            over = (w.abs() - b > 65520).to(DEV)
+            assert torch.equal(a[over], w.to(dtype).to(DEV)[over]) and bool(a[over].isinf().all())
+            a, w, b = (torch.where(over.to(t.device) | ((w.abs() + b).to(t.device) > 65504), 0, t) for t in (a, w, b))
+        near(a, w, b + 1e-36, what)
+    h, new = gated_recurrence_step(v[:, 0], g[:, 0], h0)
+    one = ref_shut(v[:, :1], g[:, :1], h0, dh[:, :1], dlast)
+    near(h, one[0][0][:, 0], one[0][1][:, 0], "step")
+    near(new, *one[1], "step's state")
+
+
 def test_recurrence_large_state_is_forgotten():
     """A state of 10^6 in front of values around 1, half of it forgotten a step: its rounding is
     forgotten with it, in the states and (from the other end) in the gradients."""
