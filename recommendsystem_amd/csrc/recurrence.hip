@@ -700,15 +700,16 @@ __global__ void __launch_bounds__(LC * NG, 2) rec_bwd_kernel(const RecArgs a) {
 #pragma unroll
     for (int k = K - 1; k >= 0; --k) {
       float d[V], gv[V], gg[V];
+      const bool in_k = W || t + rv_.ls + k < p.n;  // (behind the end also an infinite gradient stands still)
       E::template unpack<2>(rd[k].w, d);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         // the smaller and the larger part of x, f x and i x or the other way round
         const float w = gate_again(in[k][j]), m = fabsf(w), x = d[j] + rt[j], lo = m * x, hi = fmaf(-m, x, x);
         const bool shut = gate_shut(w);
-        gv[j] = shut ? hi : lo;
-        gg[j] = m * hi * e[k][j];
-        rt[j] = shut ? lo : hi;
+        gv[j] = !in_k ? 0.f : shut ? hi : lo;
+        gg[j] = in_k ? m * hi * e[k][j] : 0.f;
+        rt[j] = !in_k ? rt[j] : shut ? lo : hi;
       }
       if (W || t + rdv_.ls + k < a.T) {
         store8<E, PART>(rdv_.at(t, k), gv, p.nv);

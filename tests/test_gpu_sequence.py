@@ -609,6 +609,22 @@ def test_recurrence_large_state_is_forgotten():
         near(a, w, b, "large state")
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("T,D", [(5, 24), (20, 130), (50, 130), (50, 8), (200, 24), (300, 24), (1100, 8), (3000, 24)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_rows_behind_the_end_have_no_gradient(bad, T, D, dtype):
+    """An overflowed gradient of the last state reaches the steps of its channel, and none behind the end."""
+    v, g = rnd(3, T, D, dtype=dtype).requires_grad_(), rnd(3, T, D, dtype=dtype).requires_grad_()
+    lengths = torch.tensor([T - 2, 0, T // 2], device=DEV)
+    h, last = gated_recurrence(v, g, None, lengths)
+    dlast = rnd(3, D)
+    dlast[:, 1] = bad
+    for grad in torch.autograd.grad((h, last), (v, g), (rnd(3, T, D, dtype=dtype), dlast)):
+        for b, n in enumerate(lengths.tolist()):
+            assert not grad[b, n:].any() and not grad[b, n:].isnan().any()
+            assert n == 0 or not grad[b, n - 1, 1].isfinite()
+
+
 def test_recurrence_nan_stays_in_its_channel():
     v, g = rnd(2, 100, 20), rnd(2, 100, 20)
     v[0, 50, 3] = float("nan")
