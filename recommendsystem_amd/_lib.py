@@ -320,20 +320,12 @@ def run_on(index: int, fn, *args):
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
-try:  # half of torch.empty's host time; the same caching allocator
-    from torch._C._dynamo.guards import _empty_strided_cuda as _empty_strided
-except ImportError:
-    def _empty_strided(shape, stride, dtype):
-        return torch.empty_strided(shape, stride, dtype=dtype, device="cuda")
+_CURRENT = torch.device("cuda")  # whichever is current
 
 
 def empty(shape, dtype=torch.float32):
     """An uninitialised contiguous tensor on the current device (inside run_on)."""
-    shape, stride, n = tuple(shape), (), 1
-    for size in reversed(shape):
-        stride = (n, *stride)
-        n *= size or 1
-    return _empty_strided(shape, stride, dtype)
+    return torch.empty(shape, dtype=dtype, device=_CURRENT)
 
 
 def device_index(ref, *others) -> int:

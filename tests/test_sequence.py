@@ -269,6 +269,15 @@ def test_encoder_traced_for_serving(custom_ops, save_8bit):
         assert y.shape == (3, 24) and states.shape == (2, 3, 16)
 
 
+def test_allocations_are_seen():
+    """Outputs and workspaces are made through torch's dispatcher: modes (memory filled in deterministic
+    runs, fake tensors, trackers) see them."""
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    with FakeTensorMode():
+        t = _lib.empty((2, 3), torch.int8)
+    assert isinstance(t, FakeTensor) and t.shape == (2, 3) and t.dtype == torch.int8 and t.is_contiguous()
+
+
 def test_dense_flag_defaults_off():
     assert not Dense(3).save_8bit and Dense(3, save_8bit=True).save_8bit
     assert packing.scale_shape((2, 129)) == (2, 2)
