@@ -350,7 +350,7 @@ def gated_recurrence_step(v, g=None, state=None, out=None):
     """One step for B sessions: v, g [B, D] (g None: v [B, 2 D]), state [B, D] float32 (None:
     zeros) -> (h [B, D] in the rows' type, the new state [B, D] float32).  out: where the new
     state goes (a contiguous float32 [B, D]; may be `state` itself, which is then updated in
-    place).  Under autograd use gated_recurrence, of which this is the case T = 1."""
+    place; overlaps no other argument).  Under autograd use gated_recurrence, of which this is the case T = 1."""
     code = _check_rec(v, g, 2, "gated_recurrence_step")
     B, D = v.shape if g is not None else (v.shape[0], v.shape[1] // 2)
     _check_state(state, (B, D), "gated_recurrence_step: state")
@@ -364,7 +364,24 @@ def gated_recurrence_step(v, g=None, state=None, out=None):
     if _lib.CUSTOM_OPS["on"]:
         h, new = torch.ops.ctr.gated_recurrence_step(v, g, state)
         return h, new if out is None else out.copy_(new)
+    if out is not None:
+        _check_out(out, v, g, state)
     return run_on(index, _rec_step, v, g, state, out, B, D, code)
+
+
+def _check_out(out, v, g, state):
+    """The step writes out while other threads still read: it may be the state itself (every element
+    is read and written by one thread), but not overlap anything otherwise."""
+    begin = out.data_ptr()
+    end = begin + 4 * out.numel()
+    for name, t in (("the values", v), ("the gates", g), ("the state", state)):
+        if t is None or t is out or not t.numel():
+            continue
+        at = t.data_ptr()
+        if at >= end or (name == "the state" and (at == begin or not t.is_contiguous())):  # (copied first)
+            continue
+        if begin < at + ((t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + 1) * t.element_size():
+            raise ValueError(f"gated_recurrence_step: out overlaps {name}")
 
 
 def _rec_step(v, g, state, out, B, D, code, stream):

@@ -675,6 +675,18 @@ def test_step_matches_the_recurrence(dtype):
     assert h.shape == (0, D)
 
 
+def test_step_output_that_overlaps_is_refused():
+    m, v = torch.zeros(96, device=DEV), rnd(5, 8)
+    state, out = m[:40].view(5, 8), m[8:48].view(5, 8)
+    with pytest.raises(ValueError, match="overlaps the state"):
+        gated_recurrence_step(v, v, state, out)
+    with pytest.raises(ValueError, match="overlaps the values"):
+        gated_recurrence_step(out, v, None, out.view(5, 8))
+    h, new = gated_recurrence_step(v, v, state, state.view(5, 8))     # another tensor of the same memory
+    assert new.data_ptr() == state.data_ptr() and torch.equal(state, h)
+    gated_recurrence_step(v, v, state, m[40:80].view(5, 8))
+
+
 # ============================================================================================
 # streams, graphs, large tensors
 # ============================================================================================

@@ -269,6 +269,20 @@ def test_encoder_traced_for_serving(custom_ops, save_8bit):
         assert y.shape == (3, 24) and states.shape == (2, 3, 16)
 
 
+def test_step_output_must_not_overlap():
+    m = torch.zeros(100)
+    state, out = m[:40].view(5, 8), m[8:48].view(5, 8)
+    v = E(5, 8)
+    for bad in ((out, v, v, state), (state, v, v, out), (out, m[:40].view(5, 8), v, None), (out, v, m[40:80].view(5, 8), None),
+                (out, m.view(5, 20)[:, :16], None, None), (out, out.view(5, 8), v, state), (m[39:79].view(5, 8), v, v, state)):
+        with pytest.raises(ValueError, match="overlaps"):
+            sequence._check_out(*bad)
+    for good in ((state, v, v, state), (state.view(5, 8), v, v, state), (m[40:80].view(5, 8), v, v, state),
+                 (out, v, v, None), (out, v, v, m[:80].view(5, 16)[:, ::2]), (m[40:40].view(0, 8), m[:0].view(0, 8), v[:0], None),
+                 (m[40:80].view(5, 8), m[:40].view(5, 8), m[80:].view(5, 4), None)):
+        sequence._check_out(*good)
+
+
 def test_allocations_are_seen():
     """Outputs and workspaces are made through torch's dispatcher: modes (memory filled in deterministic
     runs, fake tensors, trackers) see them."""
