@@ -269,7 +269,8 @@ def gather_multi(src, plans):
 
 
 class _DenseFn(torch.autograd.Function):
-    """save_8bit: x is kept for the backward as pack8's codes and scales."""
+    """save_8bit: x is kept for the backward as pack8's codes and scales, or not at all where neither
+    the kernel nor the bias wants a gradient."""
 
     @staticmethod
     def forward(ctx, x, W, b, act, sink=None, save_8bit=False):
@@ -280,7 +281,10 @@ class _DenseFn(torch.autograd.Function):
         y = torch.empty(M, N, device=x.device, dtype=torch.float32)
         call("rs_dense_fwd", stream_handle(), ptr(x), M, K, x.stride(0), ptr(W), ptr(b), N, act,
              ptr(y), N)
-        ctx.save_for_backward(*(pack8(x) if save_8bit else (x, None)), y, W, b)
+        kept = (x, None)
+        if save_8bit:
+            kept = pack8(x) if W.requires_grad or b.requires_grad else (None, None)
+        ctx.save_for_backward(*kept, y, W, b)
         ctx.act = act
         ctx.sink = sink
         return y
@@ -291,12 +295,11 @@ class _DenseFn(torch.autograd.Function):
         if scales is not None:
             x = unpack8(x, scales)
         dy = _row_major(dy)
-        M, K = x.shape
-        N = W.shape[1]
+        M, (K, N) = dy.shape[0], W.shape
         s = stream_handle()
         ws_n = int(_lib.load().rs_dense_bwd_weight_workspace_floats(M, K, N))
-        ws = torch.empty(ws_n, device=x.device, dtype=torch.float32)
-        in_place = W.grad is not None and b.grad is not None and W.grad.is_contiguous()
+        ws = torch.empty(ws_n if x is not None else 0, device=dy.device, dtype=torch.float32)
+        in_place = x is None or W.grad is not None and b.grad is not None and W.grad.is_contiguous()
         dW = W.grad if in_place else torch.empty_like(W)
         db = b.grad if in_place else torch.empty_like(b)
         dx = None
@@ -306,9 +309,13 @@ class _DenseFn(torch.autograd.Function):
                 raise RuntimeError(f"GradSink holds a {tuple(sink.buf.shape)} gradient for a Dense "
                                    f"input of {(M, K)}: the producer's gradient would be lost")
             acc = sink is not None and sink.buf is not None
-            dx = sink.buf if acc else torch.empty(M, K, device=x.device, dtype=torch.float32)
+            dx = sink.buf if acc else torch.empty(M, K, device=dy.device, dtype=torch.float32)
             if sink is not None:
                 sink.buf = None
+            if x is None:
+                call("rs_dense_bwd_data", s, ptr(dy), dy.stride(0), ptr(y), N, ctx.act, ptr(W), M, K, N,
+                     ptr(dx), K, 1 if acc else 0)
+                return dx, None, None, None, None, None
             call("rs_dense_bwd", s, ptr(x), x.stride(0), ptr(dy), dy.stride(0), ptr(y), N, ctx.act,
                  ptr(W), M, K, N, ptr(dx), K, 1 if acc else 0, ptr(dW), ptr(db),
                  1 if in_place else 0, ptr(ws), ws_n)
@@ -434,9 +441,10 @@ class _GroupedDenseFn(torch.autograd.Function):
 def grouped_dense(layers, xs):
     """[layer_i(x_i)] for built Dense layers of one input rank, as ONE grouped launch per pass
     (same math as calling each layer; the per-expert / per-task loops of staytime/VideoDnn.py and
-    rough_rank/layer.py).  Up to 8 layers per group; layers with save_8bit run one by one."""
+    rough_rank/layer.py).  Up to 8 layers per group; in training, layers with save_8bit run one by
+    one."""
     layers, xs = list(layers), list(xs)
-    if len(layers) == 1 or len(layers) > 8 or any(l.save_8bit for l in layers):
+    if len(layers) == 1 or len(layers) > 8 or (torch.is_grad_enabled() and any(l.save_8bit for l in layers)):
         return [l(x) for l, x in zip(layers, xs)]
     for l, x in zip(layers, xs):
         if not l.built:

@@ -829,6 +829,40 @@ def test_dense_save_8bit():
     assert bool((err <= step.t() @ dz.abs().float() * 1.001 + 1e-4).all())
 
 
+def test_dense_save_8bit_packs_only_for_a_kernel_gradient(monkeypatch):
+    """A frozen layer passes its input's gradient on without its input, and its gradient buffers are left
+    alone; a forward without any gradient, and a group of layers in inference, keep nothing either."""
+    from recommendsystem_amd import layers
+    packed = []
+    monkeypatch.setattr(layers, "pack8", lambda x: (packed.append(1), pack8(x))[1])
+    a, b = Dense(20, "relu", seed=3), Dense(20, "relu", seed=3, save_8bit=True)
+    x, dy = rnd(65, 300), rnd(65, 20)
+    xa, xb = x.clone().requires_grad_(), x.clone().requires_grad_()
+    a(xa).backward(dy)
+    y = b(x)
+    assert len(packed) == 1                   # (its parameters want gradients)
+    for p in b.parameters():
+        p.requires_grad_(False)
+    grads = [t.grad.fill_(7.0) for t in (b.kernel, b.bias)]
+    assert torch.equal(b(xb), y)
+    b(xb).backward(dy)
+    dz = dy.double() * (y > 0)
+    near(xb.grad, (dz @ a.kernel.detach().double().t()).cpu(), 64 * U * (dz.abs() @ a.kernel.detach().double().abs().t()).cpu(), "dx")
+    near(xa.grad, (dz @ a.kernel.detach().double().t()).cpu(), 64 * U * (dz.abs() @ a.kernel.detach().double().abs().t()).cpu(), "dx")
+    assert all(bool((t == 7.0).all()) for t in grads) and not b(x).requires_grad
+    sink = layers.GradSink()                  # the producer's gradient is added onto
+    sink.buf = dx = rnd(65, 300)
+    want = dx.double().cpu() + xb.grad.double().cpu()
+    xs = x.clone().requires_grad_()
+    b(xs, sink).backward(dy)
+    near(xs.grad, want, 4 * U * (want.abs() + xb.grad.double().cpu().abs()), "dx onto a sink's")
+    c = Dense(20, "relu", seed=4, save_8bit=True)
+    with torch.no_grad():
+        for got, layer in zip(layers.grouped_dense([b, c], [x, x]), (b, c)):
+            near(got, layer(x).double().cpu(), 64 * U * (x.double().abs() @ layer.kernel.double().abs()).cpu(), "grouped")
+    assert len(packed) == 1
+
+
 def plain_encoder(enc, x, lengths, states, dtype=torch.float64):
     """SequenceEncoder from elementary operations in float64, for autograd on the CPU."""
     p = {k: t.detach().cpu().to(dtype).requires_grad_() for k, t in enc.named_parameters()}
