@@ -22,6 +22,8 @@ import torch
 from recommendsystem_amd import (Dense, GatedRecurrence, LayerNormalization, SequenceEncoder,
                                  gated_recurrence, gated_recurrence_step, layer_norm, pack8, unpack8)
 
+from _rec_forms import FORMS
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 U = 2.0 ** -24
@@ -410,6 +412,14 @@ def test_recurrence_segments_that_end_anywhere(B, T, D):
                                    (150, 600, 40), (90, 600, 130)])
 def test_gated_recurrence_narrow(B, T, D, dtype, ragged):
     """Few channels: one or two tiles of 32 bytes, with and without a cut time axis, and widths just above."""
+    test_gated_recurrence(B, T, D, dtype, ragged)
+
+
+@pytest.mark.parametrize("ragged", [False, True], ids=["", "ragged"])
+@pytest.mark.parametrize("dtype,B,T,D", [pytest.param(t, *shape[3:], id="-".join(map(str, (names(t), *shape))))
+                                         for t in TYPES for shape in FORMS[t.itemsize]])
+def test_gated_recurrence_forms(B, T, D, dtype, ragged):
+    """Every form of the kernels in every type (test_sequence.py holds the shapes to their forms)."""
     test_gated_recurrence(B, T, D, dtype, ragged)
 
 

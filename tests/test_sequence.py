@@ -6,6 +6,7 @@ import torch
 from recommendsystem_amd import _lib, packing, sequence
 from recommendsystem_amd import ops  # noqa: F401
 from recommendsystem_amd.layers import Dense
+from _rec_forms import FORMS, STEPS
 
 F32, BF16, F16, F64 = torch.float32, torch.bfloat16, torch.float16, torch.float64
 E = torch.empty
@@ -205,6 +206,32 @@ def test_size_queries():
     assert lib.rs_gated_rec_states_floats(0, -1, 5, 5) == 0
     assert lib.rs_gated_rec_states_floats(7, 1, 5, 5) == 0
     assert lib.rs_layernorm_bwd_workspace_floats(-1, 5) == 0
+
+
+@pytest.mark.parametrize("size, code", [(4, 0), (2, 1), (2, 2)])
+def test_recurrence_forms_are_those_named(size, code):
+    """The shapes that the kernels are tested with take the forms they are listed for: the queries give
+    the tiles and the cut.  One tile keeps no states (narrow long rows excepted); wide and long tiles are
+    then told apart by a longer history of the same batch and width."""
+    lib = _lib.load()
+
+    def tiles(B, T, D):
+        return lib.rs_gated_rec_states_floats(code, B, T, D) / (B * D)
+    for form, width, kind, B, T, D in FORMS[size]:
+        shape, n = (form, B, T, D), -(-T // STEPS[form])
+        assert (width == "part") == (D * size % 8 != 0), shape
+        assert (lib.rs_gated_rec_workspace_floats(code, B, T, D) > 0) == (kind == "cut"), shape
+        assert (n > 1) == (kind != "one"), shape
+        assert tiles(B, T, D) == (n if n > 1 or form == "slim_long" else 0), shape
+        if n == 1 and form in ("long", "wide"):
+            assert tiles(B, 1025, D) == -(-1025 // STEPS[form]), shape
+        if form in ("slim", "wave"):       # of the same length
+            assert (D * size <= 64) == (form == "slim"), shape
+    for form in STEPS:
+        for width in ("-", "part"):
+            kinds = {"flat": {"many"}, "short": {"one"}, "wave": {"one", "many"}, "slim": {"many"},
+                     "slim_long": {"many", "cut"}}.get(form, {"one", "many", "cut"})
+            assert {k for f, w, k, *_ in FORMS[size] if (f, w) == (form, width)} == kinds
 
 
 def test_size_queries_of_empty_batches():
