@@ -328,6 +328,11 @@ def empty(shape, dtype=torch.float32):
     return torch.empty(shape, dtype=dtype, device=_CURRENT)
 
 
+def empty_as(t, dtype=None):
+    """The same of t's shape, and type unless given (half the host time of empty(t.shape))."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def device_index(ref, *others) -> int:
     """The ROCm device that every tensor (None allowed after the first) is on."""
     index = ref.get_device()

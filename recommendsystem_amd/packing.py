@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import call, device_index, empty, run_on
+from ._lib import call, device_index, empty, empty_as, run_on
 
 BLOCK = 128
 ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -56,7 +56,7 @@ def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _pack(x, D, code, stream):
     x2 = rows_of(x)
-    codes, scales = empty(x.shape, torch.int8), empty(scale_shape(x.shape))
+    codes, scales = empty_as(x, torch.int8), empty(scale_shape(x.shape))
     call("rs_pack8", stream, code, x2.data_ptr(), x2.stride(0), x2.shape[0], D, codes.data_ptr(),
          scales.data_ptr())
     return codes, scales
@@ -77,7 +77,7 @@ def unpack8(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.float32) -> t
 
 def _unpack(codes, scales, D, dtype, stream):
     codes, scales = codes.contiguous(), scales.contiguous()
-    y = empty(codes.shape, dtype)
+    y = empty_as(codes, dtype)
     call("rs_unpack8", stream, ELEMENT_TYPES[dtype], codes.data_ptr(), scales.data_ptr(),
          codes.numel() // D, D, y.data_ptr(), D)
     return y

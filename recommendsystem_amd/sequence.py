@@ -26,7 +26,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, device_index, empty, ptr, run_on
+from ._lib import call, device_index, empty, empty_as, ptr, run_on
 from .layers import Dense
 from .packing import element_code, pack8, rows_of, scale_shape, unpack8  # noqa: F401
 from .params import FlatBlock, grads_contiguous
@@ -85,12 +85,12 @@ def _check_norm(x, gamma, beta, epsilon):
 def _norm_forward(x, gamma, beta, epsilon, code, stats, save_8bit, stream):
     x2 = rows_of(x)
     R, D = x2.shape
-    y = empty(x.shape, x.dtype)
+    y = empty_as(x)
     mean = codes = scales = None  # mean: [means | 1 / standard deviations]
     if stats:
         mean = empty((2, R))
     if save_8bit:
-        codes, scales = empty(x.shape, torch.int8), empty(scale_shape(x.shape))
+        codes, scales = empty_as(x, torch.int8), empty(scale_shape(x.shape))
     gamma, beta = gamma.contiguous(), beta.contiguous()  # (copies live until after the launch)
     call("rs_layernorm_fwd", stream, code, x2.data_ptr(), x2.stride(0), R, D, gamma.data_ptr(),
          beta.data_ptr(), epsilon, y.data_ptr(), D,
@@ -103,7 +103,7 @@ def _norm_backward(dy, x, codes, scales, gamma, mean, code, dparams, accumulate,
     dy2 = rows_of(dy)
     R, D = dy2.shape
     x2 = rows_of(x) if x is not None else None
-    dx = empty(dy.shape, dy.dtype)
+    dx = empty_as(dy)
     if dparams is None:
         dparams = empty((2, D))
     ws_n = _norm_workspace(R, D)
@@ -258,7 +258,7 @@ def _rec_forward(v, g, h0, lengths, code, keep, stream):
     v, v_sb, v_st = _strided(v)
     g, g_sb, g_st = _strided(g)
     n_states, n_ws = _rec_sizes(code, B, T, D)
-    h = empty((B, T, D), v.dtype)
+    h = empty_as(v)
     last = empty((B, D))
     states = empty((n_states,)) if keep and n_states else None
     ws = empty((n_ws,)) if n_ws else None
@@ -270,8 +270,8 @@ def _rec_forward(v, g, h0, lengths, code, keep, stream):
 def _rec_backward(v, g, h0, lengths, states, dh, dlast, code, want_h0, stream):
     """(dv, dg, dh0); with g None dv is the gradient of the joint rows and dg None."""
     joint = g is None
-    dvg = empty(v.shape, v.dtype)
-    dv, dg = _halves(dvg, None if joint else empty(v.shape, v.dtype))
+    dvg = empty_as(v)
+    dv, dg = _halves(dvg, None if joint else empty_as(v))
     v, g = _halves(v, g)
     B, T, D = v.shape
     v, v_sb, v_st = _strided(v)
@@ -390,7 +390,7 @@ def _rec_step(v, g, state, out, B, D, code, stream):
         v, g = (t if t.stride(1) == 1 else t.contiguous() for t in (v, g))
     if state is not None:
         state = state.contiguous()
-    h = empty((B, D), v.dtype)
+    h = empty_as(v)
     if out is None:
         out = empty((B, D))
     call("rs_gated_rec_step", stream, code, v.data_ptr(), v.stride(0), g.data_ptr(), g.stride(0), B, D,
