@@ -42,6 +42,19 @@ struct LnShape {
   static constexpr int RPB = THREADS / TPR;  // rows a workgroup holds at a time
 };
 
+// dy gamma, rounded: as part of an fma it would not cancel against the mean of the rounded ones (in a
+// row of one column, whose input's gradient is zero, it has to)
+__device__ __forceinline__ float ln_weighted(float y, float gm) {
+#pragma clang fp contract(off)
+  return y * gm;
+}
+// The same, computed again: kept over the row's sums the products would take as many registers as
+// the row (32768 x 2048 bf16 from 8 bits: 136 us, 86 so)
+__device__ __forceinline__ float ln_weighted_again(float y, float gm) {
+  asm("" : "+v"(y));
+  return ln_weighted(y, gm);
+}
+
 // sums of v[0..N) over the TPR threads of a row, in each of them.  red: two buffers of N floats a
 // wave, used in turn (flip), so one barrier a call is enough.
 template <int N, int TPR>
@@ -227,7 +240,7 @@ __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_bwd_kernel(const LnA
       const int nv = a.D - (c * TPR + tr) * V;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float w = y[c][j] * gm[c][j];
+        const float w = ln_weighted(y[c][j], gm[c][j]);
         x[c][j] = j < nv ? x[c][j] - mean : 0.f;
         s[0] += w;
         s[1] = fmaf(w, x[c][j], s[1]);
@@ -244,7 +257,7 @@ __global__ void __launch_bounds__(LnShape<TPR>::THREADS) ln_bwd_kernel(const LnA
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float d = x[c][j] - dl;
-        o[j] = rs * (fmaf(y[c][j], gm[c][j], -c1) - d * c2);
+        o[j] = rs * fmaf(-d, c2, ln_weighted_again(y[c][j], gm[c][j]) - c1);
         if (live) {  // (the last row again must not add its NaN to another's zeros)
           ag[c][j] = fmaf(y[c][j], d * rs, ag[c][j]);
           ab[c][j] += y[c][j];
@@ -417,7 +430,7 @@ __global__ void __launch_bounds__(LN_WIDE) ln_wide_bwd_kernel(const LnArgs a) {
       ln_in<E, Q8>(a, nb, r, col, x);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float w = y[j] * gm[j], d = j < nv ? x[j] - m : 0.f;
+        const float w = ln_weighted(y[j], gm[j]), d = j < nv ? x[j] - m : 0.f;
         s[0] += w;
         s[1] = fmaf(w, d, s[1]);
         s[2] += d;
@@ -431,7 +444,7 @@ __global__ void __launch_bounds__(LN_WIDE) ln_wide_bwd_kernel(const LnArgs a) {
       load_f<V>(gm, a.gamma + col, nv);
       ln_in<E, Q8>(a, nb, r, col, x);
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = rs * (fmaf(y[j], gm[j], -c1) - (x[j] - m - dl) * c2);
+      for (int j = 0; j < V; ++j) o[j] = rs * fmaf(-(x[j] - m - dl), c2, ln_weighted(y[j], gm[j]) - c1);
       store16<E>((X*)a.dx + r * a.lddx + col, o, nv);
     });
     if (threadIdx.x == 0) a.ws[r] = m + dl;

@@ -227,6 +227,23 @@ def test_layer_norm_outlier(at, D, dtype, save_8bit):
         near(got, w, bound, what)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+def test_layer_norm_of_one_column(dtype):
+    """y is beta whatever x is, so x's gradient is zero, to the last bit.  Kept in 8 bits x comes back
+    within 2 u |x| (the scale's rounding and the product's), d, and dx = -w d^2 / sd^3."""
+    x, dy = rnd(912, 1, dtype=dtype).requires_grad_(), rnd(912, 1, dtype=dtype)
+    gamma, beta = rnd(1, mean=1.0).requires_grad_(), rnd(1).requires_grad_()
+    for save_8bit in (False, True):
+        y = layer_norm(x, gamma, beta, 1e-5, save_8bit)
+        assert torch.equal(y, beta.to(dtype).expand(912, 1))
+        dx, dgamma, dbeta = torch.autograd.grad(y, (x, gamma, beta), dy)
+        d = 2 * U * x.detach().double().abs() * (save_8bit * 1.01)
+        w = (dy.double() * gamma.detach().double()).abs()
+        assert bool((dx.double().abs() <= w * d * d * 1e-5 ** -1.5).all())
+        assert float(dgamma.detach()) <= float((dy.double().abs() * d).sum()) * 1e-5 ** -0.5
+        near(dbeta, dy.double().cpu().sum(0), 256 * U * dy.double().cpu().abs().sum(0), "dbeta")
+
+
 def test_layer_norm_strides_ranks_and_empty():
     gamma, beta = rnd(40, mean=1.0).requires_grad_(), rnd(40).requires_grad_()
     wide = rnd(12, 100)
