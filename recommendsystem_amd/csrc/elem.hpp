@@ -237,8 +237,10 @@ __device__ __forceinline__ void load_codes(uint32_t* w, const int8_t* p, int nv)
       if (j < nv) w[j / 4] |= (uint32_t)(uint8_t)p[j] << (8 * (j % 4));
   }
 }
+// (rounded, as rs_unpack8 gives them: not as part of an fma with what is done to them next)
 template <int V>
 __device__ __forceinline__ void unpack_codes(const uint32_t* w, float s, float* x) {
+#pragma clang fp contract(off)
 #pragma unroll
   for (int j = 0; j < V; ++j) x[j] = (float)(int8_t)(w[j / 4] >> (8 * (j % 4))) * s;
 }

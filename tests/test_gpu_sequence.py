@@ -244,6 +244,19 @@ def test_layer_norm_of_one_column(dtype):
         near(dbeta, dy.double().cpu().sum(0), 256 * U * dy.double().cpu().abs().sum(0), "dbeta")
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+def test_layer_norm_kept_values_are_those_of_unpack8(dtype):
+    """In one column all that is left of the kept value is its rounding: the gradient sees the number that
+    unpack8 gives, not a product carried on without rounding."""
+    x, dy = rnd(900, 1, dtype=dtype).requires_grad_(), rnd(900, 1, dtype=dtype)
+    gamma = rnd(1, mean=1.0).requires_grad_()
+    dgamma, = torch.autograd.grad(layer_norm(x, gamma, rnd(1), 1e-5, True), gamma, dy)
+    d = unpack8(*pack8(x)).double().cpu() - x.detach().double().cpu()
+    terms = dy.double().cpu() * d * 1e-5 ** -0.5
+    assert bool(d.any())
+    near(dgamma, terms.sum(0), 256 * U * terms.abs().sum(0), "dgamma")
+
+
 def test_layer_norm_strides_ranks_and_empty():
     gamma, beta = rnd(40, mean=1.0).requires_grad_(), rnd(40).requires_grad_()
     wide = rnd(12, 100)
