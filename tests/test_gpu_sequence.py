@@ -253,8 +253,8 @@ def test_layer_norm_kept_values_are_those_of_unpack8(dtype):
     dgamma, = torch.autograd.grad(layer_norm(x, gamma, rnd(1), 1e-5, True), gamma, dy)
     d = unpack8(*pack8(x)).double().cpu() - x.detach().double().cpu()
     terms = dy.double().cpu() * d * 1e-5 ** -0.5
-    # (the 8 bits of bf16 come back whole: fl(fl(m / 127) 127) = m for all m of 128 .. 255)
-    assert bool(d.any()) or dtype is torch.bfloat16
+    # (16-bit values mostly come back whole: fl(fl(m / 127) 127) = m for all 8-bit m, and all but 7 11-bit ones)
+    assert bool(d.any()) or dtype is not torch.float32
     near(dgamma, terms.sum(0), 256 * U * terms.abs().sum(0), "dgamma")
 
 
