@@ -890,8 +890,10 @@ int rs_layernorm_bwd(void* stream, int dtype, const void* dy, int64_t ld_dy, con
  * taken into 0..T): steps behind them are not read, h is zero there and the state stands still.
  * D and, with more than one step, step strides (*_st) of 2^23 elements or more: -2.
  * h [B, T, D] contiguous; last [B, D]: the state after lengths[b] steps.  states
- * (rs_gated_rec_states_floats, 0 for short sequences; NULL without a backward): fp32 states at
- * fixed steps, for rs_gated_rec_bwd with the same shape.  workspace: rs_gated_rec_workspace_floats floats. */
+ * (rs_gated_rec_states_floats, 0 for short sequences and for B = 0; NULL without a backward): fp32
+ * states at fixed steps, for rs_gated_rec_bwd with the same shape.  workspace:
+ * rs_gated_rec_workspace_floats floats.  Values and states are finite (an infinity gives NaN in its
+ * channel from some later step on). */
 int64_t rs_gated_rec_states_floats(int dtype, int64_t B, int64_t T, int D);
 int64_t rs_gated_rec_workspace_floats(int dtype, int64_t B, int64_t T, int D);
 int rs_gated_rec_fwd(void* stream, int dtype, const void* v, int64_t v_sb, int64_t v_st,
@@ -907,7 +909,7 @@ int rs_gated_rec_bwd(void* stream, int dtype, const void* v, int64_t v_sb, int64
                      void* dg, int64_t dg_sb, int64_t dg_st, float* dh0, float* workspace,
                      int64_t workspace_floats);
 /* One step for B tokens: v, g [B, D] (row strides ld_*), state [B, D] fp32 (NULL: zeros) ->
- * h [B, D] in the rows' type and new_state [B, D] fp32 (may be state itself). */
+ * h [B, D] in the rows' type and new_state [B, D] fp32 (may be state itself; overlaps nothing else). */
 int rs_gated_rec_step(void* stream, int dtype, const void* v, int64_t ld_v, const void* g,
                       int64_t ld_g, int64_t B, int D, const float* state, void* h,
                       float* new_state);

@@ -13,9 +13,11 @@
 // beta in registers and the next row's loads in flight.  In the backward every thread also keeps its
 // columns' share of dgamma and dbeta in registers over all of its rows; one partial row a workgroup
 // then goes to the workspace and a second launch adds them in a fixed order.
-// 65536 x 1024 bf16: forward 46 us (5.8 TB/s), backward 78 + 4 us (5.2 TB/s); a large copy of torch's
+// 65536 x 1024 bf16: forward 46 us (5.8 TB/s), backward 80 + 4 us (5.0 TB/s); a large copy of torch's
 // runs at 5.4 TB/s.  Rows that start off 16 bytes cost more, each load then touching two pieces of 64
-// bytes: 40000 x 1500 bf16 forward 5.5, backward 3.5 TB/s; 4099 x 5003 fp16 3.7 and 2.9 TB/s.
+// bytes: 40000 x 1500 bf16 forward 5.5, backward 3.5 TB/s; 4099 x 5003 fp16 3.6 and 2.9 TB/s.  Rows wider
+// than any shape are read two or three times: 4096 x 12000 fp32 forward 126 us (3.1 TB/s of what a pass
+// moves once), backward 220 (2.7); 4096 x 32768 bf16 210 (2.6) and 361 us (2.2).
 #include "elem.hpp"
 
 #define LN_MAX_D 32768

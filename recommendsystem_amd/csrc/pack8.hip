@@ -2,7 +2,8 @@
 // a block of 128 columns (the form and its rounding: elem.hpp), rs_unpack8 gives it back.
 // Bound by memory.  A block's 128 columns are 16 bytes each of 128 / V lanes of a wave (fewer for
 // narrow rows), whose largest magnitude is found by lane exchanges alone; a thread has several
-// blocks' loads in flight.  131072 x 1024 bf16: pack 76 us (5.3 TB/s), unpack 63 us (6.4 TB/s).
+// blocks' loads in flight.  131072 x 1024 bf16: pack 77 us at best and 90 in the
+// median (5.3 and 4.5 TB/s), unpack 63 us (6.4 TB/s).
 #include "elem.hpp"
 
 namespace {

@@ -28,11 +28,14 @@
 // costs a fixed number of operations a channel and thread: twice the steps a thread, half the joins.
 // Tiles that are wholly part of the sequence go through a loop of their own with nothing conditional
 // around its loads and stores: only then does the compiler know how many are in flight, and waits for
-// the next tile's loads without waiting for this tile's stores (8 x 4096 x 2048 bf16, backward: 146 us,
-// 175 us where both were waited for; 10 x 4096 x 2048: 214 against 271; 37 x 1021 x 520 fp32: 109 against 126).
-// 8 x 4096 x 2048 bf16 (256 workgroups, pieces of 128 bytes): forward 85 to 94 us (4.5 TB/s), backward
-// 146 us (4.6 TB/s).  8 x 4096 x 4096 in pieces of 256 bytes: 155 us (5.2 TB/s) and 268 us (5.0 TB/s),
-// as fast as a copy of that size.
+// the next tile's loads without waiting for this tile's stores (forward and backward, bf16, 10 x 4096 x
+// 2048: 123 and 215 us, 145 and 247 with every tile masked; 8 x 4096 x 2048: 93 and 155 against 98 and 161;
+// 37 x 1021 x 520 fp32: the same).  Widths that are no multiple of 8 bytes still have such conditions
+// everywhere (PART): 8 x 4096 x 2046 bf16 takes 169 and 354 us.
+// 8 x 4096 x 2048 bf16 (256 workgroups, pieces of 128 bytes): forward 93 us (4.4 TB/s), backward 155 us
+// (4.4 TB/s).  8 x 4096 x 4096 in pieces of 256 bytes: 149 us (5.4 TB/s) and 257 us (5.2 TB/s), as fast
+// as a copy of that size.  Holding a step as the smaller of i and f costs 0 to 7 percent of this, at some
+// shapes up to 14 (10 x 4096 x 2048 bf16 forward 112 -> 123 us, 4096 x 50 x 8 backward 11.6 -> 13.4).
 #include "elem.hpp"
 
 namespace {
@@ -789,34 +792,38 @@ namespace {
 //   WIDE  128 steps x 256 bytes, 512 threads: rows are read in longer pieces, which memory likes, but
 //         it takes twice the channels for as many workgroups, and an odd number of 128 bytes leaves
 //         half of a tile beyond the width
-// Forward + backward, us, bf16 (number of 128-byte tiles):        WAVE   LONG   WIDE
-//   1024 x   50 x 1024 (16384)                                     207    770    433
-//    256 x  256 x 1024 (4096)                                      220    253    253
-//    128 x  512 x  512 (1024)                                      111    125    112
-//     64 x 1024 x 2048 (2048)                                      479    447    426
-//     12 x 4096 x 2048 (384)                                       414    373    353
-//     60 x 2000 x  512 (480)                                              225    207
-//     60 x 2000 x  520 (540)                                              307    345
-//    100 x 1000 x  264 (500)                                              105    149
-//      8 x 4096 x 2048 (256)                                       266    248    272
-//     37 x  300 x  333 (222)                                        62     38     68
+// Forward + backward, us, bf16 (number of 128-byte tiles), and fp32 rows of the same bytes:
+//                                          WAVE   LONG   WIDE      WAVE   LONG   WIDE
+//   1024 x   50 x 1024 (16384)              218    959    491       193    655    350
+//    256 x  256 x 1024 (4096)               224    275    254       227    232    225
+//    128 x  512 x  512 (1024)               122    143    119       118    119    108
+//     64 x 1024 x 2048 (2048)               487    465    422       480    435    415
+//     12 x 4096 x 2048 (384)                495    393    367       410    372    342
+//     60 x 2000 x  512 (480)                262    234    205       237    222    201
+//     60 x 2000 x  520 (540)                344    331    361       335    302    329
+//    100 x 1000 x  264 (500)                145    131    185       120    112    154
+//      8 x 4096 x 2048 (256)                340    252    294       279    246    282
+//     37 x  300 x  333 (222)                 87     50     70        42     31     48
 // narrow rows                     FLAT   SLIM   SLIM_LONG   the best of the others
-//  12000 x    16 x  8               14     39
-//   5000 x    20 x 32               20     35                 28 (SHORT)
-//  20000 x    50 x  8               46     65
-//   9000 x   100 x 16               62     58
-//  40000 x    50 x 16 fp32         241    281
-//    512 x    50 x 16                       9       28        13 (WAVE)
-//     64 x   100 x 16                      12       15        14 (WAVE)
-//    512 x   300 x 16                      24       30        37 (WAVE)
-//     32 x   300 x 16                      21       15        25 (LONG)
-//    512 x  1000 x 16                      59       43        81 (LONG)
-//    256 x  4000 x 32                     198      136       156 (LONG)
-//     16 x  4000 x 32                     186       29        27 (LONG)
-//     64 x 20000 x  8                     890       92       245 (LONG)
-// Up to 128 workgroups the time axis is cut so that there are at most 256, one round (65521 x 1000
-// fp16 forward: 133 us with 16 segments, 151 with 32 in two rounds); above 128 a cut would read the
-// input twice to fill less than half of the chip more.
+//  12000 x    16 x  8               19     49      669        74 (SHORT)
+//   5000 x    20 x 32               26     43      574        38 (SHORT)
+//  20000 x    50 x  8               56     76     1137       192 (SHORT)     SLIM is taken
+//   9000 x   100 x 16               90     72      537       156 (SHORT)
+//  40000 x    50 x 16 fp32         241    286     3157       296 (SHORT)
+//    512 x    50 x 16               43     11       33        17 (WAVE)
+//     64 x   100 x 16               75     14       18        17 (LONG)
+//    512 x   300 x 16              210     28       36        50 (WAVE)
+//    512 x   300 x  8 fp32         152     24       28        36 (WAVE)
+//     32 x   300 x 16              208     25       18        29 (LONG)
+//    512 x  1000 x 16              675     67       47        97 (LONG)
+//    512 x  1000 x  8 fp32         485     56       39        67 (LONG)
+//    256 x  4000 x 32             2722    231      153       179 (LONG)
+//     16 x  4000 x 32             2673    219       35        32 (LONG)      SLIM_LONG is taken
+//     64 x 20000 x  8            13346   1057      103       299 (LONG)
+//     64 x 20000 x  4 fp32        9555    835       88       230 (LONG)
+// Up to 128 workgroups the time axis is cut so that there are at most 256, one round (1 x 65521 x 1000
+// fp16 forward, WIDE: 139 us with 32 segments, 256 workgroups; 218 with 128 workgroups, 141 with 512 in
+// two rounds); above 128 a cut would read the input twice to fill less than half of the chip more.
 enum { REC_FLAT, REC_SHORT, REC_WAVE, REC_LONG, REC_WIDE, REC_SLIM, REC_SLIM_LONG };
 struct RecPlan {
   int kind, steps;  // steps: of a time tile

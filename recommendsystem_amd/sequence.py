@@ -15,6 +15,7 @@ a served session has to keep.
     f_t = sigmoid(g_t)        h_t = f_t h_{t-1} + (1 - f_t) v_t
 
 Rows are float32, bfloat16 or float16; gamma, beta, states and the parameters' gradients float32.
+First derivatives in reverse mode only: second ones and forward mode (dual tensors) are refused.
 """
 from __future__ import annotations
 
@@ -156,7 +157,9 @@ def layer_norm(x, gamma, beta, epsilon=1e-5, save_8bit=False):
     (float32 / bfloat16 / float16, any leading shape and strides); gamma and beta float32.
     save_8bit: keep x for the backward in 8 bits (packing.py) instead of as it is; y, mean and
     variance are those of x itself, and so is the sum of dy; the normalised rows that dx and
-    dgamma are computed with are those of the kept values."""
+    dgamma are computed with are those of the kept values.
+    Sums are float32: a row whose squared deviations sum past its range (deviations of 1e18 or
+    so) gives beta."""
     return _norm(x, gamma, beta, float(epsilon), bool(save_8bit), False)
 
 
@@ -331,7 +334,11 @@ def gated_recurrence(v, g=None, h0=None, lengths=None):
     lengths int32 / int64 [B]: steps from lengths[b] on are not part of the sequence (values are
     taken into 0..T): whatever v and g hold there, h is zero, no gradient flows, and the returned
     state is that after lengths[b] steps (h0 for an empty sequence).
-    v, g: float32 / bfloat16 / float16, any strides (unit along D is read in place)."""
+    v, g: float32 / bfloat16 / float16, any strides (unit along D is read in place).
+    The smaller of f and 1 - f is held to its own digits, to some 2^-21 of itself for float32 rows; for
+    16-bit rows the exponential's argument is rounded too, |g| 2^-24 more, which h does not show but
+    the float32 state and h0's gradient carry.  Values and states have to be finite: an infinity
+    gives NaN in its channel from the same step on or a later one, where the formula would stay infinite."""
     code = _check_rec(v, g, 3, "gated_recurrence")
     B, T, D = v.shape if g is not None else (*v.shape[:2], v.shape[2] // 2)
     _check_state(h0, (B, D), "gated_recurrence: h0")
