@@ -453,7 +453,6 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
   typedef Rows<E, LC, NG, K, const X*> In;
   const In rv_((const X*)a.v, p.b, a.v_sb, a.v_st, p.cl), rg_((const X*)a.g, p.b, a.g_sb, a.g_st, p.cl);
   const Rows<E, LC, NG, K, X*> rh_((X*)a.h, p.b, a.T * a.D, a.D, p.c0);
-  const int64_t some = p.n > 0 ? p.n : 1;  // steps that may be read
   const int64_t ch = p.b * a.D + p.c0;
   const int t0 = p.seg * a.tps, t1 = min(a.tiles, t0 + a.tps);
 
@@ -471,8 +470,8 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
     const int64_t t = wave_step<LC, NG, K>(tile);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, some), p.nv);
-      load8<E, PART>(ng_[k], W ? rg_.at(t, k) : rg_.in(t, k, some), p.nv);
+      load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, p.n), p.nv);
+      load8<E, PART>(ng_[k], W ? rg_.at(t, k) : rg_.in(t, k, p.n), p.nv);
     }
   };
   // one tile; next: starts the next tile's loads, in between
@@ -522,7 +521,7 @@ __global__ void __launch_bounds__(LC * NG) rec_fwd_kernel(const RecArgs a) {
   };
   // whole tiles up to tw, then those with the sequence's end inside, up to te, then nothing to read
   const int tw = NG == 1 ? t0 : max(t0, (int)min((int64_t)t1, p.n / STEPS));
-  const int te = NG == 1 ? t1 : (int)min((int64_t)t1, (p.n + STEPS - 1) / STEPS);
+  const int te = (int)min((int64_t)t1, (p.n + STEPS - 1) / STEPS);
   if (tw > t0 + 1) {
     // (the first by itself: the loop then starts with as many stores in flight as it goes on with)
     load(t0, Yes());
@@ -622,7 +621,6 @@ __global__ void __launch_bounds__(LC * NG, 2) rec_bwd_kernel(const RecArgs a) {
   const In rv_((const X*)a.v, p.b, a.v_sb, a.v_st, p.cl), rg_((const X*)a.g, p.b, a.g_sb, a.g_st, p.cl),
       rd_((const X*)(none ? a.g : a.dh), p.b, none ? a.g_sb : a.dh_sb, none ? a.g_st : a.dh_st, p.cl);
   const Out rdv_((X*)a.dv, p.b, a.dv_sb, a.dv_st, p.c0), rdg_((X*)a.dg, p.b, a.dg_sb, a.dg_st, p.c0);
-  const int64_t some = p.n > 0 ? p.n : 1;  // steps that may be read
   const int64_t ch = p.b * a.D + p.c0;
   const int t0 = p.seg * a.tps, t1 = min(a.tiles, t0 + a.tps);
 
@@ -631,7 +629,7 @@ __global__ void __launch_bounds__(LC * NG, 2) rec_bwd_kernel(const RecArgs a) {
   for (int j = 0; j < V; ++j) r[j] = 0.f;
   if (a.dlast) load_n<V, PART>(r, a.dlast + ch, p.nv);
   // tiles wholly behind the sequence's end: nothing to read
-  const int te = NG == 1 ? t1 : (int)min((int64_t)t1, (p.n + STEPS - 1) / STEPS);
+  const int te = (int)min((int64_t)t1, (p.n + STEPS - 1) / STEPS);
   if (NG > 1 && p.seg + 1 < a.segs)
     segment_fold<E, LC, NG, PART, false>(a, p, p.seg + 1, a.segs, ch, r, lds[te & 1]);
 
@@ -646,9 +644,9 @@ __global__ void __launch_bounds__(LC * NG, 2) rec_bwd_kernel(const RecArgs a) {
     else if (a.h0) load_n<V, PART>(ns, a.h0 + ch, p.nv);  // one tile
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      load8<E, PART>(ng_[k], W ? rg_.at(t, k) : rg_.in(t, k, some), p.nv);
-      load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, some), p.nv);
-      load8<E, PART>(nd_[k], W ? rd_.at(t, k) : rd_.in(t, k, some), p.nv);
+      load8<E, PART>(ng_[k], W ? rg_.at(t, k) : rg_.in(t, k, p.n), p.nv);
+      load8<E, PART>(nv_[k], W ? rv_.at(t, k) : rv_.in(t, k, p.n), p.nv);
+      load8<E, PART>(nd_[k], W ? rd_.at(t, k) : rd_.in(t, k, p.n), p.nv);
     }
   };
   // one tile; next: starts the loads of the tile in front, in between
